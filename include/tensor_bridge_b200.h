@@ -84,8 +84,9 @@ const char* tb_last_error(void);
 /* TB_OK if `device` is an sm_100 GPU this library was built for. */
 tb_status tb_device_supported(int device);
 
-/* Read (and optionally clear) the error word that kernels set when a bounded
- * device-side wait expires.  Synchronises the device.  *code = 0 means none. */
+/* Read (and optionally clear) the error word that kernels set: bit 0 when a
+ * bounded device-side wait expires, bits 1 and 2 by the cache's kernels (see
+ * tb_kv4_rows).  Synchronises the device.  *code = 0 means none. */
 tb_status tb_device_error(int* code, int clear);
 
 /* ---- decode streamers ---------------------------------------------------- */
@@ -295,6 +296,104 @@ tb_status tb_gemm_i8(const int8_t* A, const int8_t* B, int32_t* D, int M, int N,
 tb_status tb_gemm_fp8_fused_int8(const uint8_t* A, const uint8_t* B, int32_t* D, int M, int N, int K, float scale,
                                  void* workspace, size_t workspace_bytes, tb_stream_t stream);
 size_t tb_gemm_fp8_fused_int8_workspace(int M, int N, int K);
+
+/* ---- key/value cache in block-scaled FP4 ---------------------------------
+ *
+ * No reference counterpart: the reference stores weights in 4 bits; these
+ * calls store an attention layer's keys and values in the same block-scaled
+ * layout (tb_decode_nvfp4's) and attend over them.
+ *
+ * The cache is an array of pages.  A page holds page_size tokens of every KV
+ * head; within it the heads follow one another, and a head's block is
+ *   [K codes: page_size x D/2][K scales: page_size x D/16]
+ *   [V codes: page_size x D/2][V scales: page_size x D/16]      (D = head_dim)
+ * with E2M1 codes packed as TB_FMT_E2M1 (first value in the HIGH nibble) and
+ * one E4M3 scale byte per 16 values, so x = e2m1 * e4m3 * k_scale (v_scale).
+ * tb_decode_nvfp4 reads either part of a block as it lies. */
+typedef struct tb_kv4_cache {
+    void* data;         /* device, 16-byte aligned */
+    size_t page_stride; /* bytes from page to page, a multiple of 16; 0: tb_kv4_page_bytes */
+    int num_pages;
+    int page_size;      /* tokens: a power of two, 16 to 1024 */
+    int kv_heads;
+    int head_dim;       /* a multiple of 16 up to 256; tb_kv4_attention: 64 or 128 */
+    float k_scale;      /* per-tensor scales, 2^-100 to 2^100 */
+    float v_scale;
+} tb_kv4_cache;
+
+/* The rows of a call and where their tokens are.  Row cu_rows[b] + i belongs
+ * to sequence b: it is token number seq_lens[b] - n + i, with
+ * n = cu_rows[b+1] - cu_rows[b]: a sequence's rows are its last n tokens, and
+ * seq_lens counts them.  Token t is in page block_table[b][t / page_size].
+ * The three arrays are on the device and read when the kernels run, so a
+ * captured call follows their contents.  cu_rows does not decrease; rows from
+ * cu_rows[batch] to `rows` belong to nobody (a padded batch): they are not
+ * read and what would be written to them stays as it was.  Table entries
+ * behind a sequence's last page are not read.
+ * Contents that the host cannot check are checked on the device: a row whose
+ * token number is negative or whose page is not in [0, num_pages) or not in
+ * the table is left out (not written, not read back, not seen by attention;
+ * an attention row of negative token number sees nothing), rows outside `rows`
+ * are not touched, and bit 1 of tb_device_error's word is set (not by
+ * attention for negative token numbers alone). */
+typedef struct tb_kv4_rows {
+    const int32_t* cu_rows;     /* device [batch + 1] */
+    const int32_t* seq_lens;    /* device [batch] */
+    const int32_t* block_table; /* device [batch x table_width] */
+    int batch;
+    int table_width;            /* table_width * page_size < 2^31 - 4096 */
+    int rows;                   /* rows that the K, V, q and out arrays hold */
+} tb_kv4_rows;
+
+/* Bytes of a page: page_size * kv_heads * head_dim * 9 / 8. */
+size_t tb_kv4_page_bytes(int page_size, int kv_heads, int head_dim);
+
+/* Quantise the rows' keys and values (fmt F16 or BF16) into the cache.  k and
+ * v hold [rows x kv_heads x head_dim], k_stride and v_stride elements from row
+ * to row (0: dense; a multiple of 8), 16-byte aligned.  Per 16 values x of a
+ * head and with g = k_scale (v_scale):
+ *   scale byte  the E4M3 value s nearest to max|x| / (6 g), a tie to the
+ *               smaller, at most 448; 0x7F (NaN) if any x is a NaN
+ *   code        the E2M1 value nearest to x / (g s), a tie to the smaller
+ *               magnitude, at most 6 (infinities too), with x's sign bit;
+ *               zero codes where s is 0 or NaN
+ * decided exactly, without rounding.  Tokens of the same page that the call
+ * does not write stay as they are.  Two rows of one call must not name the
+ * same place in the cache (two sequences that share the page they write to):
+ * what is then held there is either row's, or a mixture. */
+tb_status tb_kv4_append(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_format fmt, const void* k,
+                        long long k_stride, const void* v, long long v_stride, tb_stream_t stream);
+
+/* Read the rows' keys and values back (fmt F16 or BF16): the product
+ * e2m1 * e4m3 * scale in FP32, rounded to the output type.  Arrays as in
+ * tb_kv4_append.  A whole sequence is read with cu_rows the running sum of
+ * seq_lens. */
+tb_status tb_kv4_read(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_format fmt, void* k, long long k_stride,
+                      void* v, long long v_stride, tb_stream_t stream);
+
+/* Attention of the rows over their sequences' cached tokens.  q and out hold
+ * [rows x q_heads x head_dim] in fmt (F16 or BF16), 16-byte aligned, q_stride
+ * and out_stride elements from row to row (0: dense; a multiple of 8); they
+ * may be the same array only if they are the same rows exactly.  Query head h
+ * reads KV head h / (q_heads / kv_heads).  The row of token number p sees
+ * token j if j <= p and (window == 0 or j > p - window or j < sinks); its own
+ * token is in the cache (tb_kv4_append comes first).  Over the tokens seen,
+ *   out = sum_j e^{s_j} v_j / sum_j e^{s_j},   s_j = softmax_scale * q . k_j
+ *   lse = ln sum_j e^{s_j}            (device [rows x q_heads] FP32, or NULL)
+ * A row that sees nothing, or only scores of -inf, has out = 0, lse = -inf.
+ * max_rows is at least the rows of any sequence (with fewer, bit 2 of
+ * tb_device_error's word is set and rows may be missing); max_len is the
+ * longest sequence, and only steers how the work is split.  The result does
+ * not depend on the order in which CTAs run.  `workspace` is device memory of
+ * tb_kv4_attention_workspace bytes for the same arguments on the current
+ * device (may be NULL if that is 0); it holds nothing between calls, and calls
+ * that may overlap in time need one each. */
+tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_format fmt, const void* q,
+                           long long q_stride, void* out, long long out_stride, float* lse, int q_heads, int max_rows,
+                           int max_len, float softmax_scale, int window, int sinks, void* workspace,
+                           size_t workspace_bytes, tb_stream_t stream);
+size_t tb_kv4_attention_workspace(const tb_kv4_cache* cache, const tb_kv4_rows* rows, int q_heads, int max_rows,
+                                  int max_len);
 
 /* ---- column-sharded weight GEMM over NCCL -------------------------------- */
 /* The reference is single-GPU; this is the B200 addition for weights too large

@@ -71,11 +71,39 @@ def stored_bytes(fmt: Format, n: int) -> int:
     return (n * num + den - 1) // den
 
 
+class KV4Cache(ctypes.Structure):
+    """tb_kv4_cache: a paged key/value cache in block-scaled FP4.  `data` is a
+    torch tensor (kept alive by this object) or a device address."""
+    _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_size_t), ("num_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
+
+    def __init__(self, data, num_pages: int, page_size: int, kv_heads: int, head_dim: int, k_scale: float = 1.0,
+                 v_scale: float = 1.0, page_stride: int = 0):
+        super().__init__(_ptr(data), page_stride, num_pages, page_size, kv_heads, head_dim, k_scale, v_scale)
+        self._keep = data
+
+
+class KV4Rows(ctypes.Structure):
+    """tb_kv4_rows: which sequences a call's rows belong to and where their
+    tokens are.  The three index arrays are int32 torch tensors (kept alive by
+    this object) or device addresses."""
+    _fields_ = [("cu_rows", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("batch", ctypes.c_int), ("table_width", ctypes.c_int), ("rows", ctypes.c_int)]
+
+    def __init__(self, cu_rows, seq_lens, block_table, batch: int, table_width: int, rows: int):
+        super().__init__(_ptr(cu_rows), _ptr(seq_lens), _ptr(block_table), batch, table_width, rows)
+        self._keep = (cu_rows, seq_lens, block_table)
+
+
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
 _f = ctypes.c_float
+_ll = ctypes.c_longlong
 _st = ctypes.c_int  # tb_status
+_kvc = ctypes.POINTER(KV4Cache)
+_kvr = ctypes.POINTER(KV4Rows)
 
 # name -> (restype, argtypes); the set of names is exactly the header's.
 SIGNATURES = {
@@ -107,6 +135,11 @@ SIGNATURES = {
     "tb_gemm_i8": (_st, [_p, _p, _p, _i, _i, _i, _p]),
     "tb_gemm_fp8_fused_int8": (_st, [_p, _p, _p, _i, _i, _i, _f, _p, _sz, _p]),
     "tb_gemm_fp8_fused_int8_workspace": (_sz, [_i, _i, _i]),
+    "tb_kv4_page_bytes": (_sz, [_i, _i, _i]),
+    "tb_kv4_append": (_st, [_kvc, _kvr, _i, _p, _ll, _p, _ll, _p]),
+    "tb_kv4_read": (_st, [_kvc, _kvr, _i, _p, _ll, _p, _ll, _p]),
+    "tb_kv4_attention": (_st, [_kvc, _kvr, _i, _p, _ll, _p, _ll, _p, _i, _i, _i, _f, _i, _i, _p, _sz, _p]),
+    "tb_kv4_attention_workspace": (_sz, [_kvc, _kvr, _i, _i, _i]),
     "tb_gemm_sharded_fused": (_st, [_i, _p, _p, _p, _i, _i, _i, _i, _f, _p, _i, _p, _p]),
     "tb_gemm_sharded_fused_p2p": (_st, [_i, _p, _p, _p, _i, _i, _i, _i, _f, _i, _p]),
     "tb_peer_buffer_register": (_st, [_p, _p, _sz, _p, ctypes.POINTER(_p)]),
@@ -252,6 +285,37 @@ def device_error(clear: bool = True) -> int:
     code = ctypes.c_int(0)
     call("tb_device_error", ctypes.byref(code), 1 if clear else 0)
     return code.value
+
+
+# ---- key/value cache in block-scaled FP4 -------------------------------------------------
+
+def kv4_page_bytes(page_size: int, kv_heads: int, head_dim: int) -> int:
+    return lib().tb_kv4_page_bytes(page_size, kv_heads, head_dim)
+
+
+def kv4_append(cache: KV4Cache, rows: KV4Rows, fmt, k, v, k_stride: int = 0, v_stride: int = 0, stream=None):
+    """Quantise the rows' keys and values (F16 or BF16) into the cache; strides
+    in elements from row to row, 0 for dense rows."""
+    call("tb_kv4_append", cache, rows, int(fmt), _ptr(k), k_stride, _ptr(v), v_stride, _stream(stream))
+
+
+def kv4_read(cache: KV4Cache, rows: KV4Rows, fmt, k, v, k_stride: int = 0, v_stride: int = 0, stream=None):
+    """The rows' cached keys and values as F16 or BF16."""
+    call("tb_kv4_read", cache, rows, int(fmt), _ptr(k), k_stride, _ptr(v), v_stride, _stream(stream))
+
+
+def kv4_attention_workspace(cache: KV4Cache, rows: KV4Rows, q_heads: int, max_rows: int, max_len: int) -> int:
+    return lib().tb_kv4_attention_workspace(cache, rows, q_heads, max_rows, max_len)
+
+
+def kv4_attention(cache: KV4Cache, rows: KV4Rows, fmt, q, out, lse, q_heads: int, max_rows: int, max_len: int,
+                  softmax_scale: float, window: int = 0, sinks: int = 0, q_stride: int = 0, out_stride: int = 0,
+                  workspace=None, workspace_bytes: int = 0, stream=None):
+    """Causal attention of the rows over the cache: all earlier tokens, or with
+    window > 0 the last `window` of them and the sequence's first `sinks`.
+    lse (FP32 [rows x q_heads]) may be None."""
+    call("tb_kv4_attention", cache, rows, int(fmt), _ptr(q), q_stride, _ptr(out), out_stride, _ptr(lse), q_heads,
+         max_rows, max_len, softmax_scale, window, sinks, _ptr(workspace), workspace_bytes, _stream(stream))
 
 
 # ---- column-sharded weight GEMM (tb_gemm_sharded_fused) -------------------------------

@@ -101,10 +101,12 @@ tb_status tb_device_error(int* code, int clear) {
     int v = 0;
     s = from_cuda(tb::device_error_read(&v), "read device error word");
     if (s != TB_OK) return s;
-    *code = v;
-    if (clear && v) {
-        s = from_cuda(tb::device_error_clear(), "clear device error word");
-    }
+    int kv4 = 0;
+    s = from_cuda(tb::kv4_device_error_read(&kv4), "read the cache kernels' error word");
+    if (s != TB_OK) return s;
+    *code = v | kv4;
+    if (clear && v) s = from_cuda(tb::device_error_clear(), "clear device error word");
+    if (clear && kv4 && s == TB_OK) s = from_cuda(tb::kv4_device_error_clear(), "clear the cache kernels' error word");
     return s;
 }
 

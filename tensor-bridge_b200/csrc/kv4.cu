@@ -1,0 +1,314 @@
+// kv4.cu -- the key/value cache in block-scaled FP4: argument checks and
+// launches of tb_kv4_append, tb_kv4_read and tb_kv4_attention.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdio>
+#include <cuda_runtime.h>
+#include "tensor_bridge_b200.h"
+#include "tb_host.h"
+#include "kv4_step_kernel.cuh"
+
+namespace {
+
+using namespace tb;
+
+tb_status refuse(tb_status s, const char* what) { return set_last_error(s, "kv4", what); }
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+size_t head_bytes(const tb_kv4_cache* c) {
+    return static_cast<size_t>(c->page_size) * static_cast<size_t>(c->head_dim) * 9 / 8;
+}
+
+// The cache's description, checked.
+tb_status check_cache(const tb_kv4_cache* c, Kv4Cache* out) {
+    if (!c) return refuse(TB_ERR_INVALID_ARGUMENT, "cache is NULL");
+    if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+        return refuse(TB_ERR_SHAPE, "page_size must be a power of two from 16 to 1024");
+    if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16)
+        return refuse(TB_ERR_SHAPE, "head_dim must be a multiple of 16 up to 256");
+    if (c->kv_heads < 1 || c->kv_heads > 65535 || c->num_pages < 0)
+        return refuse(TB_ERR_SHAPE, "kv_heads must be 1 to 65535 and num_pages not negative");
+    const size_t least = head_bytes(c) * static_cast<size_t>(c->kv_heads);
+    const size_t stride = c->page_stride ? c->page_stride : least;
+    if (stride < least) return refuse(TB_ERR_SHAPE, "page_stride is less than the page's bytes");
+    if (stride % 16) return refuse(TB_ERR_ALIGNMENT, "page_stride must be a multiple of 16 bytes");
+    // Also keeps every border of the quantiser an ordinary FP32 number.
+    const float least_scale = 0x1p-100f, most_scale = 0x1p100f;
+    if (!(c->k_scale >= least_scale && c->k_scale <= most_scale && c->v_scale >= least_scale &&
+          c->v_scale <= most_scale))
+        return refuse(TB_ERR_INVALID_ARGUMENT, "k_scale and v_scale must lie between 2^-100 and 2^100");
+    if (!c->data && c->num_pages) return refuse(TB_ERR_INVALID_ARGUMENT, "cache data is NULL");
+    if (!aligned16(c->data)) return refuse(TB_ERR_ALIGNMENT, "cache data must be 16-byte aligned");
+    out->data = static_cast<uint8_t*>(c->data);
+    out->page_stride = stride;
+    out->num_pages = c->num_pages;
+    out->page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+    out->heads = c->kv_heads;
+    out->dim = c->head_dim;
+    out->k_scale = c->k_scale;
+    out->v_scale = c->v_scale;
+    return TB_OK;
+}
+
+tb_status check_rows(const tb_kv4_rows* r, int page_shift, Kv4Rows* out) {
+    if (!r) return refuse(TB_ERR_INVALID_ARGUMENT, "rows is NULL");
+    if (r->batch < 0 || r->rows < 0 || r->table_width < 0) return refuse(TB_ERR_SHAPE, "negative batch, rows or table_width");
+    if ((static_cast<long long>(r->table_width) << page_shift) > 0x7FFFFFFFll - 4096)
+        return refuse(TB_ERR_SHAPE, "table_width * page_size must stay below 2^31 - 4096");
+    if (r->batch && r->rows && (!r->cu_rows || !r->seq_lens || (!r->block_table && r->table_width)))
+        return refuse(TB_ERR_INVALID_ARGUMENT, "cu_rows, seq_lens or block_table is NULL");
+    out->cu = r->cu_rows;
+    out->lens = r->seq_lens;
+    out->table = r->block_table;
+    out->batch = r->batch;
+    out->width = r->table_width;
+    out->rows = r->rows;
+    return TB_OK;
+}
+
+tb_status check_type(tb_format fmt) {
+    return fmt == TB_FMT_F16 || fmt == TB_FMT_BF16 ? TB_OK : refuse(TB_ERR_INVALID_ARGUMENT, "rows must be F16 or BF16");
+}
+
+// Row stride in elements: 0 stands for dense rows.
+tb_status check_stride(long long* stride, long long least) {
+    if (*stride == 0) *stride = least;
+    if (*stride < least) return refuse(TB_ERR_SHAPE, "a row stride is less than a row");
+    if (*stride % 8) return refuse(TB_ERR_ALIGNMENT, "a row stride must be a multiple of 8 elements");
+    return TB_OK;
+}
+
+tb_status check_gpu(int* sms) {
+    const int dev = current_device();
+    const tb_status s = tb_device_supported(dev);
+    if (s == TB_OK) *sms = device_info(dev).sms;
+    return s;
+}
+
+tb_status launched(cudaError_t e) {
+    return e == cudaSuccess ? TB_OK : refuse(TB_ERR_LAUNCH, cudaGetErrorString(e));
+}
+
+tb_status check_copy(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_format fmt, const void* k,
+                     long long k_stride, const void* v, long long v_stride, Kv4Copy* a, int* sms) {
+    tb_status s = check_cache(cache, &a->cache);
+    if (s == TB_OK) s = check_rows(rows, a->cache.page_shift, &a->rows);
+    if (s == TB_OK) s = check_type(fmt);
+    const long long width = static_cast<long long>(cache && s == TB_OK ? cache->kv_heads : 0) * a->cache.dim;
+    if (s == TB_OK) s = check_stride(&k_stride, width);
+    if (s == TB_OK) s = check_stride(&v_stride, width);
+    if (s != TB_OK) return s;
+    if (a->rows.batch == 0 || a->rows.rows == 0) return TB_OK;
+    if (!k || !v) return refuse(TB_ERR_INVALID_ARGUMENT, "null pointer");
+    if (!aligned16(k) || !aligned16(v)) return refuse(TB_ERR_ALIGNMENT, "rows must be 16-byte aligned");
+    a->k = const_cast<void*>(k);
+    a->v = const_cast<void*>(v);
+    a->k_stride = k_stride;
+    a->v_stride = v_stride;
+    return check_gpu(sms);
+}
+
+// A CTA of few rows starts fastest and spreads a step's rows over the SMs; one
+// of many rows has enough loads in flight.  The change is made where the small
+// CTAs would be more than the SMs hold at once (8 of 256 threads each).
+bool many_rows(const Kv4Copy& a, int per_cta, int sms, unsigned* y) {
+    const int pairs = 2 * a.cache.heads;
+    *y = static_cast<unsigned>((pairs + kKv4CopyThreads / 32 - 1) / (kKv4CopyThreads / 32));
+    return static_cast<long long>((a.rows.rows + per_cta - 1) / per_cta) * *y > 8ll * sms;
+}
+
+dim3 copy_grid(const Kv4Copy& a, int per_cta, unsigned y) {
+    return dim3(static_cast<unsigned>((a.rows.rows + per_cta - 1) / per_cta), y);
+}
+
+template <bool BF16>
+cudaError_t run_append(const Kv4Copy& a, cudaStream_t st, int sms) {
+    unsigned y;
+    if (many_rows(a, 4, sms, &y)) k_kv4_append<BF16, 16><<<copy_grid(a, 16, y), kKv4CopyThreads, 0, st>>>(a);
+    else k_kv4_append<BF16, 4><<<copy_grid(a, 4, y), kKv4CopyThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <bool BF16>
+cudaError_t run_read(const Kv4Copy& a, cudaStream_t st, int sms) {
+    unsigned y;
+    if (many_rows(a, 4, sms, &y)) k_kv4_read<BF16, 32, 8><<<copy_grid(a, 32, y), kKv4CopyThreads, 0, st>>>(a);
+    else k_kv4_read<BF16, 4, 2><<<copy_grid(a, 4, y), kKv4CopyThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+// ---- attention -----------------------------------------------------------------------
+
+// What a call's sizes alone decide.
+struct AttnPlan {
+    int nt;         // step kernel: tiles of 8 rows
+    int max_tiles;
+    int whole;
+    int runs;
+    int min_run;
+    size_t bytes;
+};
+
+AttnPlan plan_attention(int heads, int dim, int group, int max_rows, int max_len, int sms) {
+    AttnPlan p{};
+    const long long rows = static_cast<long long>(max_rows) * group;
+    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    const int tile = 8 * p.nt;
+    p.max_tiles = static_cast<int>((rows + tile - 1) / tile);
+    p.whole = max_len <= 1024;
+    p.runs = sms * (p.nt == 1 ? 2 : 1);
+    p.min_run = 2 * kStepWarps;
+    p.bytes = p.whole ? 0 : static_cast<size_t>(p.runs) * 2 * tile * (dim + 2) * sizeof(float);
+    (void)heads;
+    return p;
+}
+
+template <class K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+    const uint64_t bit = 1ull << (current_device() & 63);
+    if (done.load() & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit);
+    return e;
+}
+
+template <int D, int NT, bool BF16>
+cudaError_t run_step(const Kv4Attn& a, cudaStream_t st) {
+    using C = StepCfg<D, NT>;
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(k_kv4_step<C, BF16>, C::SMEM, done);
+    if (e != cudaSuccess) return e;
+    const unsigned units = static_cast<unsigned>(a.rows.batch) * a.cache.heads * a.max_tiles;
+    k_kv4_step<C, BF16><<<a.whole ? units : a.runs, kStepWarps * 32, C::SMEM, st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || a.whole) return e;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(units);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_kv4_join<C, BF16>, a);
+}
+
+template <int D, bool BF16>
+cudaError_t run_attention(const Kv4Attn& a, int nt, cudaStream_t st) {
+    if (nt == 1) return run_step<D, 1, BF16>(a, st);
+    if (nt == 2) return run_step<D, 2, BF16>(a, st);
+    return run_step<D, 4, BF16>(a, st);
+}
+
+tb_status check_heads(const tb_kv4_cache* c, int q_heads, int max_rows, int max_len) {
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return refuse(TB_ERR_SHAPE, "attention needs a head_dim of 64 or 128");
+    if (q_heads < 1 || q_heads % c->kv_heads) return refuse(TB_ERR_SHAPE, "q_heads must be a multiple of kv_heads");
+    if (max_rows < 0 || max_len < 0) return refuse(TB_ERR_SHAPE, "negative max_rows or max_len");
+    return TB_OK;
+}
+
+}  // namespace
+
+cudaError_t tb::kv4_device_error_read(int* v) { return cudaMemcpyFromSymbol(v, g_tb_device_error, sizeof(int)); }
+
+cudaError_t tb::kv4_device_error_clear() {
+    const int zero = 0;
+    return cudaMemcpyToSymbol(g_tb_device_error, &zero, sizeof zero);
+}
+
+extern "C" {
+
+size_t tb_kv4_page_bytes(int page_size, int kv_heads, int head_dim) {
+    if (page_size < 1 || kv_heads < 1 || head_dim < 1) return 0;
+    return static_cast<size_t>(page_size) * head_dim * 9 / 8 * kv_heads;
+}
+
+tb_status tb_kv4_append(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_format fmt, const void* k,
+                        long long k_stride, const void* v, long long v_stride, tb_stream_t stream) {
+    Kv4Copy a{};
+    int sms = 0;
+    const tb_status s = check_copy(cache, rows, fmt, k, k_stride, v, v_stride, &a, &sms);
+    if (s != TB_OK || a.rows.batch == 0 || a.rows.rows == 0) return s;
+    a.lanes_per_row = static_cast<uint32_t>(a.cache.dim) / 16;
+    a.magic = (65536u + a.lanes_per_row - 1) / a.lanes_per_row;
+    return launched(fmt == TB_FMT_BF16 ? run_append<true>(a, stream, sms) : run_append<false>(a, stream, sms));
+}
+
+tb_status tb_kv4_read(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_format fmt, void* k, long long k_stride,
+                      void* v, long long v_stride, tb_stream_t stream) {
+    Kv4Copy a{};
+    int sms = 0;
+    const tb_status s = check_copy(cache, rows, fmt, k, k_stride, v, v_stride, &a, &sms);
+    if (s != TB_OK || a.rows.batch == 0 || a.rows.rows == 0) return s;
+    a.lanes_per_row = static_cast<uint32_t>(a.cache.dim) / 8;
+    a.magic = (65536u + a.lanes_per_row - 1) / a.lanes_per_row;
+    return launched(fmt == TB_FMT_BF16 ? run_read<true>(a, stream, sms) : run_read<false>(a, stream, sms));
+}
+
+size_t tb_kv4_attention_workspace(const tb_kv4_cache* cache, const tb_kv4_rows* rows, int q_heads, int max_rows,
+                                  int max_len) {
+    Kv4Cache c{};
+    Kv4Rows r{};
+    if (check_cache(cache, &c) != TB_OK || check_rows(rows, c.page_shift, &r) != TB_OK) return 0;
+    if (check_heads(cache, q_heads, max_rows, max_len) != TB_OK) return 0;
+    return plan_attention(c.heads, c.dim, q_heads / c.heads, max_rows, max_len, device_info(current_device()).sms).bytes;
+}
+
+tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_format fmt, const void* q,
+                           long long q_stride, void* out, long long out_stride, float* lse, int q_heads, int max_rows,
+                           int max_len, float softmax_scale, int window, int sinks, void* workspace,
+                           size_t workspace_bytes, tb_stream_t stream) {
+    Kv4Attn a{};
+    tb_status s = check_cache(cache, &a.cache);
+    if (s == TB_OK) s = check_rows(rows, a.cache.page_shift, &a.rows);
+    if (s == TB_OK) s = check_type(fmt);
+    if (s == TB_OK) s = check_heads(cache, q_heads, max_rows, max_len);
+    if (s != TB_OK) return s;
+    if (static_cast<long long>(a.rows.rows) * q_heads > 0x7FFFFFFFll / 2)
+        return refuse(TB_ERR_SHAPE, "rows * q_heads must stay below 2^30");
+    if (window < 0 || sinks < 0) return refuse(TB_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
+    if (!std::isfinite(softmax_scale)) return refuse(TB_ERR_INVALID_ARGUMENT, "softmax_scale must be finite");
+    const long long width = static_cast<long long>(q_heads) * a.cache.dim;
+    s = check_stride(&q_stride, width);
+    if (s == TB_OK) s = check_stride(&out_stride, width);
+    if (s != TB_OK) return s;
+    if (a.rows.batch == 0 || a.rows.rows == 0 || max_rows == 0) return TB_OK;
+    if (!q || !out) return refuse(TB_ERR_INVALID_ARGUMENT, "null pointer");
+    if (!aligned16(q) || !aligned16(out)) return refuse(TB_ERR_ALIGNMENT, "q and out must be 16-byte aligned");
+    a.q = q;
+    a.out = out;
+    a.lse = lse;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.q_heads = q_heads;
+    a.group = q_heads / a.cache.heads;
+    a.scale_log2 = softmax_scale * a.cache.k_scale * 1.4426950408889634f;
+    a.window = window;
+    a.sinks = sinks;
+    int sms = 0;
+    s = check_gpu(&sms);
+    if (s != TB_OK) return s;
+    const AttnPlan p = plan_attention(a.cache.heads, a.cache.dim, a.group, std::min(max_rows, a.rows.rows), max_len, sms);
+    if (p.bytes) {
+        if (!workspace || workspace_bytes < p.bytes) return refuse(TB_ERR_WORKSPACE, "workspace missing or too small");
+        if (!aligned16(workspace)) return refuse(TB_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    }
+    a.ws = static_cast<float*>(workspace);
+    a.whole = p.whole;
+    a.max_tiles = p.max_tiles;
+    a.runs = p.runs;
+    a.min_run = p.min_run;
+    if (static_cast<long long>(a.rows.batch) * a.cache.heads * a.max_tiles > 0x7FFFFFFFll)
+        return refuse(TB_ERR_SHAPE, "batch * kv_heads * row tiles must stay below 2^31");
+    const bool bf16 = fmt == TB_FMT_BF16;
+    cudaError_t e;
+    if (a.cache.dim == 128) e = bf16 ? run_attention<128, true>(a, p.nt, stream) : run_attention<128, false>(a, p.nt, stream);
+    else e = bf16 ? run_attention<64, true>(a, p.nt, stream) : run_attention<64, false>(a, p.nt, stream);
+    return launched(e);
+}
+
+}  // extern "C"

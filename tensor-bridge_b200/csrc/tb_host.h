@@ -77,6 +77,10 @@ tb_status gemm_fused_to_peers(tb_format a_fmt, const void* A, const uint16_t* B,
 cudaError_t device_error_read(int* v);
 cudaError_t device_error_clear();
 
+// kv4.cu: the error word of the cache's kernels, a translation unit's own.
+cudaError_t kv4_device_error_read(int* v);
+cudaError_t kv4_device_error_clear();
+
 // api.cu: record "<what>: <detail>" as the calling thread's last error and
 // return `s` (for entry points defined outside api.cu).
 tb_status set_last_error(tb_status s, const char* what, const char* detail);
