@@ -7,7 +7,7 @@
 #include <cuda_runtime.h>
 #include "tensor_bridge_b200.h"
 #include "tb_host.h"
-#include "kv4_step_kernel.cuh"
+#include "kv4_prompt_kernel.cuh"
 
 namespace {
 
@@ -143,25 +143,32 @@ cudaError_t run_read(const Kv4Copy& a, cudaStream_t st, int sms) {
 
 // What a call's sizes alone decide.
 struct AttnPlan {
-    int nt;         // step kernel: tiles of 8 rows
-    int max_tiles;
-    int whole;
-    int runs;
-    int min_run;
-    size_t bytes;
+    int nt;             // step kernel: tiles of 8 rows
+    int whole, runs, min_run;
+    size_t step_bytes;  // of its partial results
+    int prompt_tiles;   // 0: no sequence has more rows than the step kernel takes
+    int splits;
+    size_t bytes;       // of both kernels' partial results
 };
 
-AttnPlan plan_attention(int heads, int dim, int group, int max_rows, int max_len, int sms) {
+AttnPlan plan_attention(int batch, int heads, int dim, int group, int max_rows, int max_len, int sms) {
     AttnPlan p{};
     const long long rows = static_cast<long long>(max_rows) * group;
     p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    const int tile = 8 * p.nt;
-    p.max_tiles = static_cast<int>((rows + tile - 1) / tile);
     p.whole = max_len <= 1024;
     p.runs = sms * (p.nt == 1 ? 2 : 1);
     p.min_run = 2 * kStepWarps;
-    p.bytes = p.whole ? 0 : static_cast<size_t>(p.runs) * 2 * tile * (dim + 2) * sizeof(float);
-    (void)heads;
+    p.step_bytes = p.whole ? 0 : static_cast<size_t>(p.runs) * 2 * (8 * p.nt) * (dim + 2) * sizeof(float);
+    p.splits = 1;
+    p.bytes = p.step_bytes;
+    if (rows > kStepRowsMost) {
+        p.prompt_tiles = static_cast<int>((rows + kPromptRows - 1) / kPromptRows);
+        // Fewer units than SMs: a unit's tokens are shared, 512 at least to each.
+        const long long units = static_cast<long long>(batch) * heads * p.prompt_tiles;
+        p.splits = static_cast<int>(std::max(1ll, std::min(sms / std::max(units, 1ll), max_len / 512ll)));
+        if (p.splits > 1)
+            p.bytes += static_cast<size_t>(units) * p.splits * kPromptRows * (dim + 2) * sizeof(float);
+    }
     return p;
 }
 
@@ -174,33 +181,54 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
     return e;
 }
 
+// Launch that may begin while the kernel before it ends.
+template <class K>
+cudaError_t launch_early(K kernel, unsigned grid, int threads, int smem, cudaStream_t st, const Kv4Attn& a) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 template <int D, int NT, bool BF16>
 cudaError_t run_step(const Kv4Attn& a, cudaStream_t st) {
     using C = StepCfg<D, NT>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(k_kv4_step<C, BF16>, C::SMEM, done);
     if (e != cudaSuccess) return e;
-    const unsigned units = static_cast<unsigned>(a.rows.batch) * a.cache.heads * a.max_tiles;
+    const unsigned units = static_cast<unsigned>(a.rows.batch) * a.cache.heads;
     k_kv4_step<C, BF16><<<a.whole ? units : a.runs, kStepWarps * 32, C::SMEM, st>>>(a);
     e = cudaGetLastError();
     if (e != cudaSuccess || a.whole) return e;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(units);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_kv4_join<C, BF16>, a);
+    return launch_early(k_kv4_join<C, BF16>, units, 256, 0, st, a);
+}
+
+template <int D, bool BF16>
+cudaError_t run_prompt(const Kv4Attn& a, cudaStream_t st) {
+    using C = PromptCfg<D>;
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(k_kv4_prompt<C, BF16>, C::SMEM, done);
+    if (e != cudaSuccess) return e;
+    const unsigned units = static_cast<unsigned>(a.rows.batch) * a.cache.heads * a.prompt_tiles;
+    e = launch_early(k_kv4_prompt<C, BF16>, units * a.prompt_splits, kPromptThreads, C::SMEM, st, a);
+    if (e != cudaSuccess || a.prompt_splits == 1) return e;
+    k_kv4_prompt_join<C, BF16><<<dim3(units, kPromptRows / 32), 256, 0, st>>>(a);
+    return cudaGetLastError();
 }
 
 template <int D, bool BF16>
 cudaError_t run_attention(const Kv4Attn& a, int nt, cudaStream_t st) {
     if (nt == 1) return run_step<D, 1, BF16>(a, st);
     if (nt == 2) return run_step<D, 2, BF16>(a, st);
-    return run_step<D, 4, BF16>(a, st);
+    const cudaError_t e = run_step<D, 4, BF16>(a, st);
+    return e == cudaSuccess && a.prompt_tiles ? run_prompt<D, BF16>(a, st) : e;
 }
 
 tb_status check_heads(const tb_kv4_cache* c, int q_heads, int max_rows, int max_len) {
@@ -255,7 +283,9 @@ size_t tb_kv4_attention_workspace(const tb_kv4_cache* cache, const tb_kv4_rows* 
     Kv4Rows r{};
     if (check_cache(cache, &c) != TB_OK || check_rows(rows, c.page_shift, &r) != TB_OK) return 0;
     if (check_heads(cache, q_heads, max_rows, max_len) != TB_OK) return 0;
-    return plan_attention(c.heads, c.dim, q_heads / c.heads, max_rows, max_len, device_info(current_device()).sms).bytes;
+    return plan_attention(r.batch, c.heads, c.dim, q_heads / c.heads, std::min(max_rows, r.rows), max_len,
+                          device_info(current_device()).sms)
+        .bytes;
 }
 
 tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_format fmt, const void* q,
@@ -292,18 +322,22 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     int sms = 0;
     s = check_gpu(&sms);
     if (s != TB_OK) return s;
-    const AttnPlan p = plan_attention(a.cache.heads, a.cache.dim, a.group, std::min(max_rows, a.rows.rows), max_len, sms);
+    const AttnPlan p = plan_attention(a.rows.batch, a.cache.heads, a.cache.dim, a.group,
+                                      std::min(max_rows, a.rows.rows), max_len, sms);
     if (p.bytes) {
         if (!workspace || workspace_bytes < p.bytes) return refuse(TB_ERR_WORKSPACE, "workspace missing or too small");
         if (!aligned16(workspace)) return refuse(TB_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
     }
     a.ws = static_cast<float*>(workspace);
     a.whole = p.whole;
-    a.max_tiles = p.max_tiles;
     a.runs = p.runs;
     a.min_run = p.min_run;
-    if (static_cast<long long>(a.rows.batch) * a.cache.heads * a.max_tiles > 0x7FFFFFFFll)
-        return refuse(TB_ERR_SHAPE, "batch * kv_heads * row tiles must stay below 2^31");
+    a.step_rows = 8 * p.nt;
+    a.prompt_ws = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.step_bytes);
+    a.prompt_tiles = p.prompt_tiles;
+    a.prompt_splits = p.splits;
+    if (static_cast<long long>(a.rows.batch) * a.cache.heads * std::max(p.prompt_tiles, 1) * p.splits > 0x3FFFFFFFll)
+        return refuse(TB_ERR_SHAPE, "batch * kv_heads * row tiles must stay below 2^30");
     const bool bf16 = fmt == TB_FMT_BF16;
     cudaError_t e;
     if (a.cache.dim == 128) e = bf16 ? run_attention<128, true>(a, p.nt, stream) : run_attention<128, false>(a, p.nt, stream);

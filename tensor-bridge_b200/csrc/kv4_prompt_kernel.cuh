@@ -1,0 +1,645 @@
+// kv4_prompt_kernel.cuh -- attention of many rows per sequence (a prompt, or a
+// chunk of one) over the block-scaled FP4 cache, on tcgen05.
+//
+// A CTA owns 256 packed rows (token, head of one KV head's group) as two tiles
+// of 128 and runs over their visible tokens in tiles of 128:
+//   S_t = Q_t K^T     tcgen05.mma, both operands in shared memory, S_t in TMEM
+//   P_t = 2^(S_t - m) one thread per row, S_t read from and P_t (FP16) written
+//                     to the same TMEM columns
+//   O_t += P_t V      tcgen05.mma, P_t from TMEM, V from shared memory
+// While one tile's rows take their exponentials the tensor core works for the
+// other.  K and V arrive as codes (bulk copies, one per page where a page is
+// at most a tile) and four warps turn them into FP16 operand tiles once per
+// 256 rows; a thread owns one token of the tile.
+//
+// Layout: K, V and Q tiles are [row][64 d] panels of 128-byte rows under the
+// 128-byte swizzle.  The same picture is K-major for Q K^T and, as [token][d],
+// N-major for P V, so one decoder serves both.  A byte's two codes come out of
+// the converter second value first; Q is stored in the same order, and the
+// output's columns are swapped back when they are read.
+//
+// The maximum m of a row is moved only when a score passes it by 2^8, so the
+// usual tile takes one pass: exponentials with the old m, the largest score
+// found along the way, and a second pass (with O scaled in TMEM) only if it
+// passed.  S_t of the next tile is issued behind P_t V of this one, so a row's
+// thread that sees S_t finds O_t at rest.
+//
+// TMEM (512 columns): S_0, S_1 (128 each, P in the first 64), O_0, O_1 (D each).
+#pragma once
+
+#include "kv4_step_kernel.cuh"
+
+namespace tb {
+
+constexpr int kPromptRows = 256;
+constexpr int kPromptTile = 128;                    // tokens
+constexpr int kPromptThreads = 512;                 // 8 softmax, 4 decode, MMA, loader, 2 idle warps
+
+template <int D_>
+struct PromptCfg {
+    static constexpr int D = D_;
+    static constexpr int PANELS = D / 64;
+    static constexpr int PANEL = 128 * 128;         // bytes: 128 rows of 64 FP16 values
+    static constexpr int OPERAND = PANELS * PANEL;  // a K, V or Q tile
+    static constexpr int SLOTS = 3;
+    static constexpr int TOKEN_BYTES = D / 2 + D / 16;
+    static constexpr int RAW = kPromptTile * TOKEN_BYTES * 2;
+    static constexpr int NR = 3;
+    static constexpr int OFF_SLOT = 2 * OPERAND;
+    static constexpr int OFF_RAW = OFF_SLOT + SLOTS * OPERAND;
+    static constexpr int OFF_BAR = OFF_RAW + NR * RAW;
+    static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment of the base
+    static constexpr int S_COLS = 128;
+    static constexpr int O_COL = 256;
+    static constexpr int SLOT_FLOATS = kPromptRows * (D + 2);
+};
+
+// Descriptor of an N-major operand tile (V as [token][d]): 64 values of N are
+// a 128-byte row, 8 rows of K an atom of 1024 bytes (the stride byte offset),
+// 64 more values of N a panel (the leading byte offset).
+template <class C>
+__device__ __forceinline__ uint64_t sdesc_v(uint32_t addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((C::PANEL >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+// Whether the prompt kernel takes a sequence: more packed rows than the step
+// kernel's largest tile.
+__device__ __forceinline__ bool prompt_takes(const Kv4Attn& a, const Kv4Seq& q) {
+    return static_cast<long long>(q.n) * a.group > kStepRowsMost;
+}
+
+// A CTA's unit: which rows of which sequence and head, and its share of their
+// tiles of tokens.
+struct PromptUnit {
+    Kv4Seq q;
+    Kv4Span span;
+    int b, head, row_base, row_count;
+    int first_pos, last_pos;
+    int t0, t1;  // tiles of the span
+    bool any;
+};
+
+__device__ __forceinline__ PromptUnit prompt_unit(const Kv4Attn& a, int unit, int split) {
+    PromptUnit u;
+    // The last row tiles see the most tokens: they come first.
+    const int per_tile = a.rows.batch * a.cache.heads;
+    const int tile = a.prompt_tiles - 1 - unit / per_tile;
+    const int rest = unit % per_tile;
+    u.b = rest / a.cache.heads;
+    u.head = rest - u.b * a.cache.heads;
+    u.q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[u.b], a.rows.cu[u.b + 1], a.rows.lens[u.b]);
+    u.row_base = tile * kPromptRows;
+    u.row_count = min(kPromptRows, u.q.n * a.group - u.row_base);
+    u.any = prompt_takes(a, u.q) && u.row_count > 0;
+    if (!u.any) return u;
+    u.first_pos = u.q.pos0 + u.row_base / a.group;
+    u.last_pos = u.q.pos0 + (u.row_base + u.row_count - 1) / a.group;
+    u.span = kv4_span(u.first_pos, u.last_pos, u.q.len, a.window, a.sinks, 7);
+    const int tiles = kv4_span_chunks(u.span);
+    u.t0 = static_cast<int>(static_cast<long long>(tiles) * split / a.prompt_splits);
+    u.t1 = static_cast<int>(static_cast<long long>(tiles) * (split + 1) / a.prompt_splits);
+    return u;
+}
+
+// Bit g set where granule g (16 tokens, or a page's share of the tile if that
+// is more) of the tile at token `tok0` has a page of the cache; bits of tokens
+// behind the sequence stay clear.  The whole warp calls it; lane g looks at
+// granule g.  *page is the lane's page number.
+__device__ __forceinline__ uint32_t prompt_pages(const Kv4Attn& a, const PromptUnit& u, int tok0, int* page) {
+    const int lane = threadIdx.x & 31;
+    const int shift = a.cache.page_shift, gshift = shift < 7 ? shift : 7;
+    const int tok = tok0 + (lane << gshift);
+    int p = -1;
+    const bool inside = (lane << gshift) < kPromptTile && tok < u.q.len;
+    if (inside) p = a.rows.table[static_cast<size_t>(u.b) * a.rows.width + (tok >> shift)];
+    *page = p;
+    return __ballot_sync(0xFFFFFFFFu, inside && kv4_page_ok(a.cache, p));
+}
+
+// Whether every row of the unit sees the whole tile and all of it has pages.
+__device__ __forceinline__ bool prompt_open(const Kv4Attn& a, const PromptUnit& u, int tok0, uint32_t pages) {
+    const int gshift = a.cache.page_shift < 7 ? a.cache.page_shift : 7;
+    const uint32_t all = (1u << (kPromptTile >> gshift)) - 1u;
+    return pages == all && tok0 + kPromptTile <= u.q.len && tok0 + kPromptTile - 1 <= u.first_pos &&
+           (a.window <= 0 || u.last_pos - tok0 < a.window || tok0 + kPromptTile <= a.sinks);
+}
+
+// Bits [lo, hi) of a word; lo and hi are any integers.
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+    lo = max(lo, 0);
+    hi = min(hi, 32);
+    if (lo >= hi) return 0u;
+    return (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
+}
+
+// One pass over the thread's 128 scores: p = 2^(s f - m), hidden ones 0.
+// Returns the largest s f - m; *sum gets the sum of p.
+template <bool MASKED>
+__device__ __forceinline__ float prompt_pass(uint32_t s_tmem, float f, float m, const uint32_t (&mask)[4],
+                                             uint32_t (&p)[64], float* sum) {
+    float top = -INFINITY, t0 = 0.0f, t1 = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_ld_32x32b_x32(s_tmem + 32 * c, s);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            float x0 = __uint_as_float(s[i]) * f - m, x1 = __uint_as_float(s[i + 1]) * f - m;
+            if constexpr (MASKED) {
+                x0 = (mask[c] >> i) & 1u ? x0 : -INFINITY;
+                x1 = (mask[c] >> (i + 1)) & 1u ? x1 : -INFINITY;
+            }
+            top = fmaxf(top, fmaxf(x0, x1));
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            t0 += x0;
+            t1 += x1;
+            p[16 * c + i / 2] = pack_half2(x0, x1);
+        }
+    }
+    *sum = t0 + t1;
+    return top;
+}
+
+template <class C, bool BF16>
+__global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn a) {
+    constexpr int D = C::D;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    uint64_t* raw_empty = raw_full + C::NR;
+    uint64_t* op_full = raw_empty + C::NR;
+    uint64_t* op_empty = op_full + C::SLOTS;
+    uint64_t* s_full = op_empty + C::SLOTS;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_full = p_full + 2;
+    uint64_t* q_full = o_full + 2;
+    uint64_t* drain = q_full + 2;
+    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+    volatile int* nan_seen = abort + 1;
+
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const int unit = blockIdx.x / a.prompt_splits, split = blockIdx.x - unit * a.prompt_splits;
+    const PromptUnit u = prompt_unit(a, unit, split);
+    const int tiles = u.any ? u.t1 - u.t0 : 0;
+    if (tiles == 0) {
+        grid_dep_wait();  // this grid's end implies the step kernel's
+        return;
+    }
+    const int act = u.row_count > 128 ? 2 : 1;  // tiles of rows in use
+
+    if (tid == 0) {
+        for (int i = 0; i < C::NR; ++i) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_empty[i], 4);
+        }
+        for (int i = 0; i < C::SLOTS; ++i) {
+            mbar_init(&op_full[i], 4);
+            mbar_init(&op_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+            mbar_init(&q_full[i], 4);
+        }
+        mbar_init(drain, 1);
+        fence_barrier_init();
+        *abort = 0;
+        *nan_seen = 0;
+        if (u.q.bad) atomicOr(&g_tb_device_error, kErrPage);
+        if (static_cast<long long>(u.q.n) * a.group > static_cast<long long>(a.prompt_tiles) * kPromptRows)
+            atomicOr(&g_tb_device_error, kErrRows);
+    }
+    if (warp == 12) tmem_alloc(tmem_ptr, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;
+
+    const int gshift = a.cache.page_shift < 7 ? a.cache.page_shift : 7;
+    const uint32_t gtok = 1u << gshift;
+    const uint32_t at_ks = gtok * (D / 2), at_vc = at_ks + gtok * (D / 16), at_vs = at_vc + gtok * (D / 2);
+    const uint32_t gbytes = gtok * C::TOKEN_BYTES * 2;
+
+    if (warp < 8) {
+        // ---- softmax: thread = row ----------------------------------------------------
+        const int t = warp / 4, r = tid & 127;
+        if (t < act) {
+            const int row = u.row_base + t * 128 + r;
+            const bool valid = t * 128 + r < u.row_count;
+            const int i = row / a.group;
+            const int pos = u.q.pos0 + i;
+            const int h = u.head * a.group + row - i * a.group;
+            // Q into its tile, pairs swapped; BF16 scaled as in the step kernel.
+            float f = a.scale_log2;
+            {
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                                  (u.q.first + i) * a.q_stride +
+                                                                  static_cast<long long>(h) * D);
+                float up = 1.0f, up2 = 1.0f;
+                if constexpr (BF16) {
+                    uint32_t e = 0;
+                    if (valid) {
+#pragma unroll
+                        for (int k = 0; k < D / 8; ++k) {
+                            const uint4 v = src[k];
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) e = max(e, max((w[j] >> 7) & 0xFFu, (w[j] >> 23) & 0xFFu));
+                        }
+                    }
+                    const int k = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = k > 120 ? 120 : k, k2 = k - k1;
+                    up = exp2i(k1);
+                    up2 = exp2i(k2);
+                    f = (f * exp2i(-k1)) * exp2i(-k2);
+                }
+                uint8_t* q_tile = smem + t * C::OPERAND;
+#pragma unroll
+                for (int k = 0; k < D / 8; ++k) {
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (valid) v = src[k];
+                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (BF16)
+                            w[j] = pack_half2(__uint_as_float(w[j] & 0xFFFF0000u) * up * up2,
+                                              __uint_as_float(w[j] << 16) * up * up2);
+                        else
+                            w[j] = prmt(w[j], 0u, 0x1032u);
+                    }
+                    *reinterpret_cast<uint4*>(q_tile + (k / 8) * C::PANEL + r * 128 + (((k & 7) ^ (r & 7)) << 4)) =
+                        make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[t]);
+            }
+
+            const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane offset 32 * (warp % 4)
+            const uint32_t s_tmem = tmem + quarter + t * C::S_COLS;
+            const uint32_t o_tmem = tmem + quarter + C::O_COL + t * D;
+            float m = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < tiles && ok; ++j) {
+                const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
+                int page;
+                const uint32_t pages = prompt_pages(a, u, tok0, &page);
+                const bool open = prompt_open(a, u, tok0, pages);
+                uint32_t mask[4];
+                if (!open) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int base = tok0 + 32 * c;
+                        uint32_t w = bit_range(0, min(pos + 1, u.q.len) - base);
+                        if (a.window > 0) {
+                            const int oldest = pos >= a.window ? pos - a.window + 1 : 0;
+                            w &= bit_range(oldest - base, 32) | bit_range(0, a.sinks - base);
+                        }
+                        uint32_t there = 0;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            if ((pages >> ((32 * c + 16 * k) >> gshift)) & 1u) there |= 0xFFFFu << (16 * k);
+                        mask[c] = w & there;
+                    }
+                }
+                ok = mbar_wait(&s_full[t], j & 1, abort);
+                if (!__all_sync(0xFFFFFFFFu, ok)) break;
+                tc_fence_after();
+                uint32_t p[64];
+                float sum;
+                const float m_use = m == -INFINITY ? 0.0f : m;
+                const float top = open ? prompt_pass<false>(s_tmem, f, m_use, mask, p, &sum)
+                                       : prompt_pass<true>(s_tmem, f, m_use, mask, p, &sum);
+                // The first score seen sets m; later ones move it past 2^8.
+                const bool move = m == -INFINITY ? top > -INFINITY : top > 8.0f;
+                if (__any_sync(0xFFFFFFFFu, move)) {
+                    const float m_new = move ? m_use + top : m;
+                    const float scale = move ? ex2(m - m_new) : 1.0f;
+                    m = m_new;
+                    l *= scale;
+                    const float again = m == -INFINITY ? 0.0f : m;
+                    if (open) prompt_pass<false>(s_tmem, f, again, mask, p, &sum);
+                    else prompt_pass<true>(s_tmem, f, again, mask, p, &sum);
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld_32x32b_x16(o_tmem + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * scale);
+                            tmem_st_32x32b_x16(o_tmem + c, o);
+                        }
+                    }
+                }
+                l += sum;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) w[k] = p[16 * c + k];
+                    tmem_st_32x32b_x16(s_tmem + 16 * c, w);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+            }
+
+            // ---- the rows' result --------------------------------------------------------
+            ok = mbar_wait(&o_full[t], 0, abort);
+            named_bar_sync(1, 128 + 128 * act);  // the decode warps have recorded their NaN blocks
+            if (__all_sync(0xFFFFFFFFu, ok)) {
+                tc_fence_after();
+                uint32_t nan_blocks = 0;
+                if (*nan_seen && valid) {
+                    // Rare: look at every block of V that was left out of a
+                    // partly visible tile, and put a NaN where this row sees it.
+                    for (int j = u.t0; j < u.t1; ++j) {
+                        const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
+                        for (int k = 0; k < kPromptTile; ++k) {
+                            const int tok = tok0 + k;
+                            if (tok >= u.q.len || !kv4_sees(pos, tok, a.window, a.sinks)) continue;
+                            const int pg = a.rows.table[static_cast<size_t>(u.b) * a.rows.width +
+                                                        (tok >> a.cache.page_shift)];
+                            if (!kv4_page_ok(a.cache, pg)) continue;
+                            const uint8_t* sc = a.cache.data + kv4_block_offset(a.cache, pg, u.head) +
+                                                2 * kv4_codes_bytes(a.cache) + kv4_scales_bytes(a.cache) +
+                                                (tok & ((1 << a.cache.page_shift) - 1)) * (D / 16);
+                            for (int x = 0; x < D / 16; ++x)
+                                if ((sc[x] & 0x7F) == 0x7F) nan_blocks |= 1u << x;
+                        }
+                    }
+                }
+                const bool partial = a.prompt_splits > 1;
+                float* slot = a.prompt_ws + static_cast<size_t>(blockIdx.x) * C::SLOT_FLOATS;
+                const float g = l == 0.0f ? 0.0f : a.cache.v_scale / l;
+                uint16_t* dst = static_cast<uint16_t*>(a.out) + (u.q.first + i) * a.out_stride +
+                                static_cast<long long>(h) * D;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld_32x32b_x32(o_tmem + c, o);
+                    tmem_wait_ld();
+                    if (!valid) continue;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        if ((nan_blocks >> ((c + k) / 16)) & 1u) o[k] = 0x7FC00000u;
+                    if (partial) {
+                        float* to = slot + (t * 128 + r) * D + c;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            *reinterpret_cast<uint4*>(to + k) = make_uint4(o[k + 1], o[k], o[k + 3], o[k + 2]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const float lo = l == 0.0f ? 0.0f : __uint_as_float(o[k + 2 * x + 1]) * g;
+                                const float hi = l == 0.0f ? 0.0f : __uint_as_float(o[k + 2 * x]) * g;
+                                if constexpr (BF16) {
+                                    const __nv_bfloat162 y = __floats2bfloat162_rn(lo, hi);
+                                    w[x] = *reinterpret_cast<const uint32_t*>(&y);
+                                } else {
+                                    w[x] = pack_half2(lo, hi);
+                                }
+                            }
+                            *reinterpret_cast<uint4*>(dst + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+                if (valid && partial) {
+                    slot[kPromptRows * D + t * 128 + r] = m;
+                    slot[kPromptRows * (D + 1) + t * 128 + r] = l;
+                } else if (valid && a.lse != nullptr) {
+                    a.lse[static_cast<long long>(u.q.first + i) * a.q_heads + h] =
+                        l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ---- decode: thread = token of the tile ------------------------------------------
+        const uint32_t tok = static_cast<uint32_t>(tid & 127);
+        const uint32_t g0 = (tok >> gshift) * gbytes, place = tok & (gtok - 1u);
+        uint32_t n_op = 0;
+        bool ok = true;
+        for (int j = 0; j < tiles && ok; ++j) {
+            const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
+            int page;
+            const uint32_t pages = prompt_pages(a, u, tok0, &page);
+            const bool open = prompt_open(a, u, tok0, pages);
+            const bool there = ((pages >> (tok >> gshift)) & 1u) && tok0 + static_cast<int>(tok) < u.q.len;
+            const int st = j % C::NR;
+            ok = mbar_wait(&raw_full[st], (j / C::NR) & 1, abort);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            const uint8_t* raw = smem + C::OFF_RAW + st * C::RAW + g0;
+#pragma unroll 1
+            for (int kv = 0; kv < 2; ++kv, ++n_op) {
+                const int slot = n_op % C::SLOTS;
+                ok = n_op < C::SLOTS || mbar_wait(&op_empty[slot], (n_op / C::SLOTS - 1) & 1, abort);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                uint8_t* dst = smem + C::OFF_SLOT + slot * C::OPERAND + tok * 128;
+                const uint8_t* codes = raw + (kv ? at_vc : 0u) + place * (D / 2);
+                const uint8_t* scales = raw + (kv ? at_vs : at_ks) + place * (D / 16);
+                uint32_t sc[D / 64];
+                if constexpr (D == 128) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(scales);
+                    sc[0] = v.x;
+                    sc[1] = v.y;
+                } else {
+                    sc[0] = *reinterpret_cast<const uint32_t*>(scales);
+                }
+#pragma unroll
+                for (int x = 0; x < D / 64; ++x) {
+                    if (!there) sc[x] = 0u;
+                    if (kv && !open && e4m3_nan_bits(sc[x])) {
+                        // A NaN block that some row may not see: out of the
+                        // product, and into the rows that see it at the end.
+                        *nan_seen = 1;
+                        const uint32_t n = e4m3_nan_bits(sc[x]) >> 7;  // 1 in the low bit of NaN bytes
+                        sc[x] &= ~(n * 0xFFu);
+                    }
+                }
+                // Lanes start at different 16-byte parts of their rows, so that
+                // neither the reads nor the writes of a quarter warp share a bank.
+                constexpr int PARTS = D / 32;
+#pragma unroll
+                for (int x = 0; x < PARTS; ++x) {
+                    const uint32_t part = (x + (tok >> 1)) & (PARTS - 1);
+                    const uint4 v = *reinterpret_cast<const uint4*>(codes + 16 * part);
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t s2;  // the part's two scale bytes
+                    if constexpr (D == 128) s2 = (part & 2u ? sc[1] : sc[0]) >> (16 * (part & 1u));
+                    else s2 = sc[0] >> (16 * part);
+                    const uint32_t ss = cvt_e4m3x2(static_cast<uint16_t>(s2));
+                    const uint32_t sa = prmt(ss, 0u, 0x1010u), sb = prmt(ss, 0u, 0x3232u);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        uint32_t o[4];
+                        cvt_e2m1x2_x4(w[y], o);
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) o[z] = hmul2(o[z], y < 2 ? sa : sb);
+                        const uint32_t chunk = 4 * part + y;  // 16-byte chunk of the decoded row
+                        *reinterpret_cast<uint4*>(dst + (chunk >> 3) * C::PANEL + (((chunk & 7u) ^ (tok & 7u)) << 4)) =
+                            make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&op_full[slot]);
+                    if (kv) mbar_arrive(&raw_empty[st]);
+                }
+            }
+        }
+        named_bar_sync(1, 128 + 128 * act);
+    } else if (warp == 12) {
+        // ---- tensor core ------------------------------------------------------------------
+        constexpr uint32_t idesc_s = idesc_make(0, 0, 128, 128);
+        constexpr uint32_t idesc_o = idesc_make(0, 0, 128, D) | (1u << 16);  // V is N-major
+        const uint32_t q0 = smem_addr(smem), slot0 = smem_addr(smem + C::OFF_SLOT);
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            ok = ok && mbar_wait(bar, parity, abort);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            tc_fence_after();
+            return ok;
+        };
+        auto scores = [&](int t, uint32_t op) {
+            if (elect_one()) {
+                const uint32_t kb = slot0 + (op % C::SLOTS) * C::OPERAND, qb = q0 + t * C::OPERAND;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t at = (k / 4) * C::PANEL + (k % 4) * 32;
+                    mma_f16_ss(tmem + t * C::S_COLS, sdesc_make(sdesc_lo(qb + at)), sdesc_make(sdesc_lo(kb + at)), idesc_s,
+                               k > 0);
+                }
+                mma_commit(&s_full[t]);
+            }
+            __syncwarp();
+        };
+        auto values = [&](int t, uint32_t op, bool first) {
+            if (elect_one()) {
+                const uint32_t vb = slot0 + (op % C::SLOTS) * C::OPERAND;
+#pragma unroll
+                for (int k = 0; k < kPromptTile / 16; ++k)
+                    mma_f16_ts(tmem + C::O_COL + t * D, tmem + t * C::S_COLS + 8 * k, sdesc_v<C>(vb + k * 2048), idesc_o,
+                               !(first && k == 0));
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint64_t* bar) {
+            if (elect_one()) mma_commit(bar);
+            __syncwarp();
+        };
+        for (int t = 0; t < act && ok; ++t) wait(&q_full[t], 0);
+        if (ok && wait(&op_full[0], 0)) {
+            for (int t = 0; t < act; ++t) scores(t, 0);
+            release(&op_empty[0]);
+        }
+        for (int j = 0; j < tiles && ok; ++j) {
+            const uint32_t v_op = 2 * j + 1, k_op = 2 * j + 2;
+            for (int t = 0; t < act && ok; ++t) {
+                if (t == 0 && !wait(&op_full[v_op % C::SLOTS], (v_op / C::SLOTS) & 1)) break;
+                if (!wait(&p_full[t], j & 1)) break;
+                values(t, v_op, j == 0);
+                if (t == act - 1) release(&op_empty[v_op % C::SLOTS]);
+                if (j + 1 < tiles) {
+                    if (t == 0 && !wait(&op_full[k_op % C::SLOTS], (k_op / C::SLOTS) & 1)) break;
+                    scores(t, k_op);
+                    if (t == act - 1) release(&op_empty[k_op % C::SLOTS]);
+                } else {
+                    release(&o_full[t]);
+                }
+            }
+        }
+        if (!ok) {  // let what was issued end before the tensor memory is given up
+            release(drain);
+            mbar_wait_drain(drain, 0);
+        }
+    } else if (warp == 13) {
+        // ---- loader ---------------------------------------------------------------------------
+        bool ok = true;
+        int j = 0;
+        for (; j < tiles && ok; ++j) {
+            const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
+            int page;
+            const uint32_t pages = prompt_pages(a, u, tok0, &page);
+            const int st = j % C::NR;
+            ok = j < C::NR || mbar_wait(&raw_empty[st], (j / C::NR - 1) & 1, abort);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            uint8_t* dst = smem + C::OFF_RAW + st * C::RAW;
+            const int want = min(kPromptTile, u.q.len - tok0);  // tokens that should have pages
+            const bool mine = (pages >> lane) & 1u;
+            if ((lane << gshift) < want && !mine) atomicOr(&g_tb_device_error, kErrPage);
+            if (lane == 0) mbar_arrive_expect_tx(&raw_full[st], __popc(pages) * gbytes);
+            __syncwarp();
+            if (mine) {
+                const uint8_t* src = a.cache.data + kv4_block_offset(a.cache, page, u.head);
+                uint8_t* to = dst + lane * gbytes;
+                if (a.cache.page_shift <= 7) {
+                    bulk_load(to, src, gbytes, &raw_full[st]);
+                } else {  // a tile of a larger page, part by part (lane 0 alone)
+                    const uint32_t place_in_page = static_cast<uint32_t>(tok0) & ((1u << a.cache.page_shift) - 1u);
+                    const uint32_t codes = kv4_codes_bytes(a.cache), scales = kv4_scales_bytes(a.cache);
+                    bulk_load(to, src + place_in_page * (D / 2), at_ks, &raw_full[st]);
+                    bulk_load(to + at_ks, src + codes + place_in_page * (D / 16), gtok * (D / 16), &raw_full[st]);
+                    src += codes + scales;
+                    bulk_load(to + at_vc, src + place_in_page * (D / 2), at_ks, &raw_full[st]);
+                    bulk_load(to + at_vs, src + codes + place_in_page * (D / 16), gtok * (D / 16), &raw_full[st]);
+                }
+            }
+            __syncwarp();
+        }
+        if (!ok && lane == 0)  // copies in flight end before the memory is given up
+            for (int k = max(0, j - C::NR); k < j; ++k) mbar_wait_drain(&raw_full[k % C::NR], (k / C::NR) & 1);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_relinquish();
+        tmem_dealloc(tmem, 512);
+    }
+    grid_dep_wait();
+}
+
+// Joins the splits of the prompt kernel's units, in their order.  blockIdx.y
+// takes 32 of a unit's rows.
+template <class C, bool BF16>
+__global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4Attn a) {
+    constexpr int D = C::D;
+    const PromptUnit u = prompt_unit(a, blockIdx.x, 0);
+    if (!u.any) return;
+    const int tiles = kv4_span_chunks(u.span);
+    const int r0 = blockIdx.y * 32, r1 = min(r0 + 32, u.row_count);
+    for (int x = r0 * (D / 4) + threadIdx.x; x < r1 * (D / 4); x += blockDim.x) {
+        const int r = x / (D / 4), d = 4 * (x % (D / 4));
+        float top = -INFINITY, l = 0.0f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < a.prompt_splits; ++s) {
+            if (static_cast<long long>(tiles) * s / a.prompt_splits ==
+                static_cast<long long>(tiles) * (s + 1) / a.prompt_splits)
+                continue;  // no tiles, no result
+            const float* slot = a.prompt_ws + (static_cast<size_t>(blockIdx.x) * a.prompt_splits + s) * C::SLOT_FLOATS;
+            kv4_merge(top, l, v, slot[kPromptRows * D + r], slot[kPromptRows * (D + 1) + r],
+                      *reinterpret_cast<const float4*>(slot + r * D + d));
+        }
+        kv4_store_row<BF16, D>(a, u.q.first, u.row_base + r, u.head, d, v, top, l);
+    }
+}
+
+}  // namespace tb

@@ -54,9 +54,12 @@ struct Kv4Attn {
     int window, sinks;
     float* ws;                     // partial results
     int whole;                     // step kernel: one CTA per unit, no partial results
-    int max_tiles;                 // row tiles of a (sequence, KV head) at most
     int runs;                      // CTAs that share the chunks (not `whole`)
     int min_run;                   // chunks a CTA should have at least
+    int step_rows;                 // packed rows that the step kernel takes; sequences with more are the prompt kernel's
+    float* prompt_ws;
+    int prompt_tiles;              // tiles of 256 packed rows of a sequence at most
+    int prompt_splits;             // CTAs that share a prompt unit's tokens
 };
 
 // Bit of the device error word: a sequence has more rows than max_rows.
@@ -64,6 +67,7 @@ enum : int { kErrRows = 4 };
 
 constexpr int kStepWarps = 8;
 constexpr int kStepChunk = 32;  // tokens
+constexpr int kStepRowsMost = 32;  // packed rows of a (sequence, KV head)
 
 template <int D_, int NT_>
 struct StepCfg {
@@ -129,25 +133,41 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Units and chunks of sequence b: `tiles` row tiles times the KV heads, each
-// with `chunks` chunks of tokens.
+// Adds a partial result (u, li, mi) to (v, l, top); a part that saw nothing of
+// the row has mi = -inf, li = 0 and u = 0, or NaN that stays.
+__device__ __forceinline__ void kv4_merge(float& top, float& l, float4& v, float mi, float li, float4 u) {
+    const float mt = fmaxf(top, mi);
+    const float f = top == -INFINITY ? 0.0f : ex2(top - mt), fi = mi == -INFINITY ? 0.0f : ex2(mi - mt);
+    l = l * f + li * fi;
+    v.x = v.x * f + u.x * fi;
+    v.y = v.y * f + u.y * fi;
+    v.z = v.z * f + u.z * fi;
+    v.w = v.w * f + u.w * fi;
+    top = mt;
+}
+
+// Chunks of sequence b's tokens for each KV head; 0 where it has no rows or
+// is not the step kernel's.
 struct StepSeq {
     Kv4Seq q;
     Kv4Span span;
-    int tiles, chunks;
-    __device__ __forceinline__ long long total(int heads) const {
-        return static_cast<long long>(tiles) * heads * chunks;
-    }
+    int chunks;
+    __device__ __forceinline__ long long total(int heads) const { return static_cast<long long>(heads) * chunks; }
 };
 
-template <int ROWS>
 __device__ __forceinline__ StepSeq step_seq(const Kv4Attn& a, int b) {
     StepSeq s;
     s.q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
-    s.tiles = (s.q.n * a.group + ROWS - 1) / ROWS;
     s.span = kv4_span(s.q.pos0, s.q.pos0 + s.q.n - 1, s.q.len, a.window, a.sinks, 5);
-    s.chunks = kv4_span_chunks(s.span);
+    const long long rows = static_cast<long long>(s.q.n) * a.group;
+    s.chunks = rows > 0 && rows <= a.step_rows ? kv4_span_chunks(s.span) : 0;
     return s;
+}
+
+// Reports a sequence that neither kernel takes: more rows than max_rows said.
+__device__ __forceinline__ void step_report(const Kv4Attn& a, const StepSeq& s) {
+    if (a.prompt_tiles == 0 && static_cast<long long>(s.q.n) * a.group > a.step_rows)
+        atomicOr(&g_tb_device_error, kErrRows);
 }
 
 // Sum of `v` over the CTA's threads, in every thread; `sums` has a slot per warp.
@@ -225,16 +245,19 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
     long long off = 0, left = 0;
     int my_run = blockIdx.x;
     if (a.whole) {
-        const int per = a.cache.heads * a.max_tiles;
-        b = blockIdx.x / per;
-        const int unit = blockIdx.x - b * per;
-        const StepSeq s = step_seq<ROWS>(a, b);
-        if (unit >= s.tiles * a.cache.heads) return;
-        off = static_cast<long long>(unit) * s.chunks;
+        b = blockIdx.x / a.cache.heads;
+        const StepSeq s = step_seq(a, b);
+        step_report(a, s);
+        if (s.chunks == 0) return;
+        off = static_cast<long long>(blockIdx.x - b * a.cache.heads) * s.chunks;
         left = s.chunks;
     } else {
         long long sum = 0;
-        for (int i = tid; i < a.rows.batch; i += blockDim.x) sum += step_seq<ROWS>(a, i).total(a.cache.heads);
+        for (int i = tid; i < a.rows.batch; i += blockDim.x) {
+            const StepSeq s = step_seq(a, i);
+            step_report(a, s);
+            sum += s.total(a.cache.heads);
+        }
         const long long total = block_sum(sum, sums);
         const int runs = step_runs(a, total);
         if (my_run >= runs) return;
@@ -244,7 +267,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
         long long before = 0;
         for (int b0 = 0; b0 < a.rows.batch; b0 += blockDim.x) {
             const int i = b0 + tid;
-            const long long w = i < a.rows.batch ? step_seq<ROWS>(a, i).total(a.cache.heads) : 0;
+            const long long w = i < a.rows.batch ? step_seq(a, i).total(a.cache.heads) : 0;
             long long upto = w;  // inclusive sum over the CTA's threads
             for (int d = 1; d < 32; d <<= 1) {
                 const long long o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
@@ -274,22 +297,19 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
     uint32_t used = 0;  // chunks this warp has taken through its ring
     const float thr = 8.0f;
     while (left > 0 && b < a.rows.batch) {
-        const StepSeq s = step_seq<ROWS>(a, b);
+        const StepSeq s = step_seq(a, b);
         if (off >= s.total(a.cache.heads)) {
             off -= s.total(a.cache.heads);
             ++b;
             continue;
         }
-        const int unit = static_cast<int>(off / s.chunks);
-        const int c0 = static_cast<int>(off - static_cast<long long>(unit) * s.chunks);
+        const int head = static_cast<int>(off / s.chunks);
+        const int c0 = static_cast<int>(off - static_cast<long long>(head) * s.chunks);
         const int c1 = left < s.chunks - c0 ? c0 + static_cast<int>(left) : s.chunks;
-        const int head = unit % a.cache.heads, tile = unit / a.cache.heads;
-        const int row_base = tile * ROWS;                       // first packed row of the tile
-        const int row_count = min(ROWS, s.q.n * a.group - row_base);
+        const int row_count = s.q.n * a.group;  // at most ROWS
         left -= c1 - c0;
         off += c1 - c0;
         if (tid == 0 && s.q.bad) atomicOr(&g_tb_device_error, kErrPage);
-        if (tid == 0 && s.tiles > a.max_tiles) atomicOr(&g_tb_device_error, kErrRows);
 
         // Queries in fragment order: lane (g, c) of k-step ks holds, for row
         // g, the values d = (D/4) c + 4 ks .. + 3, each pair swapped as the
@@ -298,9 +318,9 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
             uint2 v = make_uint2(0u, 0u);
             float scale = a.scale_log2;
             if (r < row_count) {
-                const int row = row_base + r, i = row / a.group;
+                const int i = r / a.group;
                 const long long at = (s.q.first + i) * a.q_stride +
-                                     static_cast<long long>(head * a.group + row - i * a.group) * D + 4 * lane;
+                                     static_cast<long long>(head * a.group + r - i * a.group) * D + 4 * lane;
                 if (lane < D / 4) v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + at);
                 if constexpr (BF16) {
                     // Exponent of the row's largest value -> 2^k that brings it to [2^14, 2^15),
@@ -352,8 +372,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
         const uint32_t at_ks = unit_tokens * (D / 2), at_vc = at_ks + unit_tokens * (D / 16),
                        at_vs = at_vc + unit_tokens * (D / 2);
         const int* table = a.rows.table + static_cast<size_t>(b) * a.rows.width;
-        const int first_pos = s.q.pos0 + row_base / a.group;                      // least and greatest position
-        const int last_pos = s.q.pos0 + (row_base + row_count - 1) / a.group;     // of the tile's rows
+        const int first_pos = s.q.pos0, last_pos = s.q.pos0 + s.q.n - 1;  // of the rows
 
         // Page numbers of a chunk: two for 16-token pages.
         auto look = [&](int q, int& p0, int& p1) {
@@ -496,8 +515,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int r = row_base + 8 * nt + 2 * c + e;
-                        const int pos = s.q.pos0 + r / a.group;
+                        const int pos = s.q.pos0 + (8 * nt + 2 * c + e) / a.group;
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -595,7 +613,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
-                                    const int pos = s.q.pos0 + (row_base + 8 * nt + 2 * c + e) / a.group;
+                                    const int pos = s.q.pos0 + (8 * nt + 2 * c + e) / a.group;
                                     if (kv4_sees(pos, tok, a.window, a.sinks))
 #pragma unroll
                                         for (int mt = 0; mt < MT; ++mt)
@@ -687,7 +705,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                     slot[ROWS * D + ROWS + r] = sum;
                 }
             } else {
-                kv4_store_row<BF16, D>(a, s.q.first, row_base + r, head, d, v, top, sum);
+                kv4_store_row<BF16, D>(a, s.q.first, r, head, d, v, top, sum);
             }
         }
         // The merge area becomes the ring again: generic accesses first.
@@ -704,40 +722,31 @@ __global__ void __launch_bounds__(256) k_kv4_join(const Kv4Attn a) {
     constexpr int D = C::D, ROWS = C::ROWS;
     __shared__ long long sums[8];
     grid_dep_wait();
-    const int per = a.cache.heads * a.max_tiles;
-    const int b = blockIdx.x / per, unit = blockIdx.x - b * per;
-    const StepSeq s = step_seq<ROWS>(a, b);
-    if (unit >= s.tiles * a.cache.heads) return;
+    const int b = blockIdx.x / a.cache.heads, head = blockIdx.x - b * a.cache.heads;
+    const StepSeq s = step_seq(a, b);
+    if (s.chunks == 0) return;
     long long sum = 0, sum_before = 0;
     for (int i = threadIdx.x; i < a.rows.batch; i += blockDim.x) {
-        const long long w = step_seq<ROWS>(a, i).total(a.cache.heads);
+        const long long w = step_seq(a, i).total(a.cache.heads);
         sum += w;
         if (i < b) sum_before += w;
     }
     const long long total = block_sum(sum, sums), before = block_sum(sum_before, sums);
     const int runs = step_runs(a, total);
-    const long long u0 = before + static_cast<long long>(unit) * s.chunks, u1 = u0 + s.chunks;
+    const long long u0 = before + static_cast<long long>(head) * s.chunks, u1 = u0 + s.chunks;
     const int r0 = static_cast<int>(((u0 + 1) * runs - 1) / total), r1 = static_cast<int>((u1 * runs - 1) / total);
     if (r0 == r1) return;  // one run had all of it
-    const int head = unit % a.cache.heads, row_base = unit / a.cache.heads * ROWS;
-    const int row_count = min(ROWS, s.q.n * a.group - row_base);
+    const int row_count = s.q.n * a.group;
     for (int x = threadIdx.x; x < row_count * (D / 4); x += blockDim.x) {
         const int r = x / (D / 4), d = 4 * (x % (D / 4));
         float top = -INFINITY, l = 0.0f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int i = r0; i <= r1; ++i) {
             const float* slot = step_slot<C>(a.ws, i, i == r0 ? 1 : 0);
-            const float mi = slot[ROWS * D + r], li = slot[ROWS * D + ROWS + r];
-            const float4 u = *reinterpret_cast<const float4*>(slot + r * D + d);
-            const float mt = fmaxf(top, mi);
-            const float f = top == -INFINITY ? 0.0f : ex2(top - mt), fi = mi == -INFINITY ? 0.0f : ex2(mi - mt);
-            // a run that saw nothing of the row has m = -inf, l = 0 and o = 0
-            l = l * f + li * fi;
-            v.x = v.x * f + u.x * fi; v.y = v.y * f + u.y * fi;
-            v.z = v.z * f + u.z * fi; v.w = v.w * f + u.w * fi;
-            top = mt;
+            kv4_merge(top, l, v, slot[ROWS * D + r], slot[ROWS * D + ROWS + r],
+                      *reinterpret_cast<const float4*>(slot + r * D + d));
         }
-        kv4_store_row<BF16, D>(a, s.q.first, row_base + r, head, d, v, top, l);
+        kv4_store_row<BF16, D>(a, s.q.first, r, head, d, v, top, l);
     }
 }
 

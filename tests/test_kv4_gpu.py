@@ -381,10 +381,20 @@ def test_prompts(tb, cuda, typ, dim, page, heads, q_heads, window, sinks):
     bt.run(q_heads, window=window, sinks=sinks)
 
 
-def test_long_prompt(tb, cuda):
-    bt = Batch(tb, cuda, [1500], [700], page=64, heads=1, dim=128, typ="bf16", seed=2)
+@pytest.mark.parametrize("page,dim", [(64, 128), (256, 64), (1024, 128), (128, 128), (16, 64)])
+def test_long_prompt(tb, cuda, page, dim):
+    """Row tiles of 256 and tokens shared by several CTAs, pages below and above the tile."""
+    bt = Batch(tb, cuda, [1500], [700], page=page, heads=1, dim=dim, typ="bf16", seed=2)
     bt.fill_fast()
     bt.run(2)
+
+
+@pytest.mark.parametrize("n", [33, 127, 128, 129, 255, 256, 257, 300])
+def test_row_tiles(tb, cuda, n):
+    """One query head per KV head: rows around the tiles of 128 and 256."""
+    bt = Batch(tb, cuda, [n, n + 77], [n, n], page=32, heads=1, dim=64, seed=n, pad=1)
+    bt.fill_fast()
+    bt.run(1)
 
 
 @pytest.mark.parametrize("n", [1, 3, 40])
