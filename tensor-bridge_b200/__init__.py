@@ -175,15 +175,30 @@ def _ptr(x):
     return x.data_ptr()
 
 
-def _stream(stream):
-    if stream is None:
+# torch's raw handle of the current device's current stream, once torch is known to have a GPU.
+_raw_stream = None
+
+
+def _current_stream():
+    global _raw_stream
+    if _raw_stream is None:
         try:
             import torch
-            if torch.cuda.is_available():
-                return torch.cuda.current_stream().cuda_stream
         except ImportError:
-            pass
-        return None
+            return None
+        if not torch.cuda.is_available():
+            return None
+        get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if get is None:
+            _raw_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
+        else:
+            _raw_stream = lambda: get(torch.cuda.current_device())  # noqa: E731
+    return _raw_stream()
+
+
+def _stream(stream):
+    if stream is None:
+        return _current_stream()
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -197,9 +212,8 @@ def _check(status: int, func: str):
 
 def call(name: str, *args):
     """Call an entry point by name and raise TBError on a non-OK status."""
-    fn = getattr(lib(), name)
-    st = fn(*args)
-    if SIGNATURES[name][0] is _st:
+    st = getattr(_lib or lib(), name)(*args)
+    if st and SIGNATURES[name][0] is _st:
         _check(st, name)
     return st
 

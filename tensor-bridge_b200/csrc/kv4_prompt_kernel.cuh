@@ -151,7 +151,7 @@ __device__ __forceinline__ float prompt_pass(uint32_t s_tmem, float f, float m, 
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-            float x0 = __uint_as_float(s[i]) * f - m, x1 = __uint_as_float(s[i + 1]) * f - m;
+            float x0 = fmaf(__uint_as_float(s[i]), f, -m), x1 = fmaf(__uint_as_float(s[i + 1]), f, -m);
             if constexpr (MASKED) {
                 x0 = (mask[c] >> i) & 1u ? x0 : -INFINITY;
                 x1 = (mask[c] >> (i + 1)) & 1u ? x1 : -INFINITY;
@@ -165,6 +165,21 @@ __device__ __forceinline__ float prompt_pass(uint32_t s_tmem, float f, float m, 
         }
     }
     *sum = t0 + t1;
+    return top;
+}
+
+// The largest s f of the thread's row that is not hidden.
+__device__ __noinline__ float prompt_top(uint32_t s_tmem, float f, const uint32_t (&mask)[4], bool open) {
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {
+        uint32_t s[16];
+        tmem_ld_32x32b_x16(s_tmem + 16 * c, s);
+        tmem_wait_ld();
+        const uint32_t w = open ? 0xFFFFu : mask[c / 2] >> (16 * (c & 1));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, (w >> i) & 1u ? __uint_as_float(s[i]) * f : -INFINITY);
+    }
     return top;
 }
 
@@ -240,7 +255,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             const int pos = u.q.pos0 + i;
             const int h = u.head * a.group + row - i * a.group;
             // Q into its tile, pairs swapped; BF16 scaled as in the step kernel.
-            float f = a.scale_log2;
+            float f = fmaxf(fabsf(a.scale_log2), 1e-37f);  // positive, its sign in q, as in the step kernel
+            const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
             {
                 const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
                                                                   (u.q.first + i) * a.q_stride +
@@ -260,7 +276,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     const int k = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = k > 120 ? 120 : k, k2 = k - k1;
                     up = exp2i(k1);
                     up2 = exp2i(k2);
-                    f = (f * exp2i(-k1)) * exp2i(-k2);
+                    f = fmaxf((f * exp2i(-k1)) * exp2i(-k2), 1e-37f);
                 }
                 uint8_t* q_tile = smem + t * C::OPERAND;
 #pragma unroll
@@ -275,6 +291,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                                               __uint_as_float(w[j] << 16) * up * up2);
                         else
                             w[j] = prmt(w[j], 0u, 0x1032u);
+                        w[j] ^= sign;
                     }
                     *reinterpret_cast<uint4*>(q_tile + (k / 8) * C::PANEL + r * 128 + (((k & 7) ^ (r & 7)) << 4)) =
                         make_uint4(w[0], w[1], w[2], w[3]);
@@ -287,7 +304,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane offset 32 * (warp % 4)
             const uint32_t s_tmem = tmem + quarter + t * C::S_COLS;
             const uint32_t o_tmem = tmem + quarter + C::O_COL + t * D;
-            float m = -INFINITY, l = 0.0f;
+            float m = kNoMax, l = 0.0f;
             bool ok = true;
             for (int j = 0; j < tiles && ok; ++j) {
                 const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
@@ -316,19 +333,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                 tc_fence_after();
                 uint32_t p[64];
                 float sum;
-                const float m_use = m == -INFINITY ? 0.0f : m;
-                const float top = open ? prompt_pass<false>(s_tmem, f, m_use, mask, p, &sum)
-                                       : prompt_pass<true>(s_tmem, f, m_use, mask, p, &sum);
-                // The first score seen sets m; later ones move it past 2^8.
-                const bool move = m == -INFINITY ? top > -INFINITY : top > 8.0f;
+                const float top = open ? prompt_pass<false>(s_tmem, f, m, mask, p, &sum)
+                                       : prompt_pass<true>(s_tmem, f, m, mask, p, &sum);
+                const bool move = top > 8.0f;
                 if (__any_sync(0xFFFFFFFFu, move)) {
-                    const float m_new = move ? m_use + top : m;
-                    const float scale = move ? ex2(m - m_new) : 1.0f;
+                    // The new m is the row's largest score, found anew: s f - m
+                    // has lost it where m was kNoMax.
+                    const float y = prompt_top(s_tmem, f, mask, open);
+                    const float m_new = move ? y : m;
+                    const float scale = ex2(m - m_new);
                     m = m_new;
                     l *= scale;
-                    const float again = m == -INFINITY ? 0.0f : m;
-                    if (open) prompt_pass<false>(s_tmem, f, again, mask, p, &sum);
-                    else prompt_pass<true>(s_tmem, f, again, mask, p, &sum);
+                    if (open) prompt_pass<false>(s_tmem, f, m, mask, p, &sum);
+                    else prompt_pass<true>(s_tmem, f, m, mask, p, &sum);
                     if (j > 0) {
 #pragma unroll 1
                         for (int c = 0; c < D; c += 16) {
@@ -628,7 +645,7 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4Attn a) {
     const int r0 = blockIdx.y * 32, r1 = min(r0 + 32, u.row_count);
     for (int x = r0 * (D / 4) + threadIdx.x; x < r1 * (D / 4); x += blockDim.x) {
         const int r = x / (D / 4), d = 4 * (x % (D / 4));
-        float top = -INFINITY, l = 0.0f;
+        float top = kNoMax, l = 0.0f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int s = 0; s < a.prompt_splits; ++s) {
             if (static_cast<long long>(tiles) * s / a.prompt_splits ==

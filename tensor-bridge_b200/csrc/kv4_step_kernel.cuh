@@ -30,12 +30,15 @@
 // as FP16: exact for values within 2^-28 of the row's largest, and off by at
 // most 2^-39 of it below, which FP32 sums do not resolve.
 //
-// Split: the (sequence, row tile, KV head) units' 32-token chunks are laid end
-// to end, and each CTA takes an equal run of them, so a batch of any lengths
-// loads all SMs alike.  A run's ends inside a unit leave partial results
-// (o, m, l) in the workspace for k_kv4_join.  Within a CTA the warps take
-// chunks in turn, each with its own ring of bulk copies and its own o, m, l,
-// merged once per unit in a fixed order.
+// Split: the (sequence, KV head) units' chunks are laid end to end, and each
+// CTA takes an equal run of them, so a batch of any lengths loads all SMs
+// alike.  A run's ends inside a unit leave partial results (o, m, l) in the
+// workspace for k_kv4_join.  Short sequences need no such plan: a cluster of
+// up to eight CTAs shares a unit and joins through distributed shared memory,
+// in one launch.  Within a CTA one warp looks pages up and issues
+// the bulk copies, a whole tile of 256 tokens by its 16 lanes at once, and
+// goes on into the next unit while eight warps compute, each on its own 32
+// tokens of a tile with its own o, m, l, merged once per unit in a fixed order.
 #pragma once
 
 #include "kv4_cache_kernel.cuh"
@@ -53,8 +56,8 @@ struct Kv4Attn {
     float scale_log2;              // softmax_scale * k_scale * log2(e)
     int window, sinks;
     float* ws;                     // partial results
-    int whole;                     // step kernel: one CTA per unit, no partial results
-    int runs;                      // CTAs that share the chunks (not `whole`)
+    int cluster;                   // step kernel: CTAs of a cluster that shares a unit; 0: runs of chunks
+    int runs;                      // CTAs that share all chunks (cluster 0)
     int min_run;                   // chunks a CTA should have at least
     int step_rows;                 // packed rows that the step kernel takes; sequences with more are the prompt kernel's
     float* prompt_ws;
@@ -65,8 +68,13 @@ struct Kv4Attn {
 // Bit of the device error word: a sequence has more rows than max_rows.
 enum : int { kErrRows = 4 };
 
-constexpr int kStepWarps = 8;
-constexpr int kStepChunk = 32;  // tokens
+constexpr int kStepWarps = 8;                        // that compute; one more loads
+constexpr int kStepThreads = 32 * (kStepWarps + 4);  // the loading warp's group of four: three of them idle
+constexpr int kStepChunk = 32;                       // tokens of a warp's share of a tile
+constexpr int kStepTile = kStepChunk * kStepWarps;
+// A row's maximum before it has seen a score: finite, so that differences are
+// ordinary numbers; every score passes it.
+constexpr float kNoMax = -1e38f;
 constexpr int kStepRowsMost = 32;  // packed rows of a (sequence, KV head)
 
 template <int D_, int NT_>
@@ -74,14 +82,22 @@ struct StepCfg {
     static constexpr int D = D_, NT = NT_;
     static constexpr int ROWS = 8 * NT;
     static constexpr int TOKEN_BYTES = D / 2 + D / 16;  // of K or of V
-    static constexpr int STAGE = kStepChunk * TOKEN_BYTES * 2;
-    static constexpr int ST = 3;
-    static constexpr int RING = kStepWarps * ST * STAGE;
-    static constexpr int MERGE = kStepWarps * ROWS * (D + 4) * 4;
-    static constexpr int QFRAG = NT * (D / 16) * 32 * 8;
-    static constexpr int UNION = RING > MERGE ? RING : MERGE;
-    static constexpr int ML = kStepWarps * ROWS * 2 * 4;
-    static constexpr int SMEM = UNION + QFRAG + ML + ROWS * 4 + kStepWarps * ST * 8 + 256;
+    static constexpr int STAGE = kStepTile * TOKEN_BYTES * 2;
+    static constexpr int ST = D == 64 ? 3 : 2;
+    static constexpr int OFF_MERGE = ST * STAGE;
+    static constexpr int OFF_Q = OFF_MERGE + kStepWarps * ROWS * (D + 4) * 4;
+    static constexpr int OFF_ML = OFF_Q + NT * (D / 16) * 32 * 8;
+    static constexpr int OFF_SCALE = OFF_ML + kStepWarps * ROWS * 2 * 4;
+    static constexpr int OFF_INFO = OFF_SCALE + ROWS * 4;
+    static constexpr int OFF_BAR = OFF_INFO + ST * kStepWarps * 8;
+    static constexpr int OFF_SUMS = OFF_BAR + 2 * ST * 8;
+    static constexpr int SMEM = OFF_SUMS + (kStepThreads / 32 + 3) * 8;
+    // Registers a thread: at launch, then of the loading group and of the
+    // computing warps.  The split never asks for more than the launch held.
+    static constexpr int CTAS = NT == 1 ? 2 : 1;
+    static constexpr int REGS = CTAS == 2 ? 80 : 168, REGS_LOAD = CTAS == 2 ? 32 : 40,
+                         REGS_COMPUTE = CTAS == 2 ? 104 : 232;
+    static_assert(128 * REGS_LOAD + 32 * kStepWarps * REGS_COMPUTE <= kStepThreads * REGS, "registers of the launch");
     static constexpr int SLOT = ROWS * (D + 2);  // floats of a partial result: o [ROWS x D], m, l
 };
 
@@ -98,6 +114,25 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
             smem_addr(smem_dst)),
         "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_addr(bar))
         : "memory");
+}
+
+// Four floats of a CTA's shared memory, by shared::cluster address.
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// Hand registers back to the CTA's pool, or take more of them (whole groups
+// of four warps; taking waits until the pool has them).
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -133,11 +168,15 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Adds a partial result (u, li, mi) to (v, l, top); a part that saw nothing of
-// the row has mi = -inf, li = 0 and u = 0, or NaN that stays.
+// log2 of the tokens of a chunk, in which sequences are split: a page's, but 32
+// at least (a warp's share) and 256 at most (a tile).
+TB_KV4_HD int step_gran(int page_shift) { return page_shift < 5 ? 5 : page_shift > 8 ? 8 : page_shift; }
+
+// Adds a partial result (u, li, mi) to (v, l, top).  A part that saw nothing
+// of the row has kNoMax, l = 0 and o = 0, or NaN, which stays.
 __device__ __forceinline__ void kv4_merge(float& top, float& l, float4& v, float mi, float li, float4 u) {
     const float mt = fmaxf(top, mi);
-    const float f = top == -INFINITY ? 0.0f : ex2(top - mt), fi = mi == -INFINITY ? 0.0f : ex2(mi - mt);
+    const float f = ex2(top - mt), fi = ex2(mi - mt);
     l = l * f + li * fi;
     v.x = v.x * f + u.x * fi;
     v.y = v.y * f + u.y * fi;
@@ -158,7 +197,7 @@ struct StepSeq {
 __device__ __forceinline__ StepSeq step_seq(const Kv4Attn& a, int b) {
     StepSeq s;
     s.q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
-    s.span = kv4_span(s.q.pos0, s.q.pos0 + s.q.n - 1, s.q.len, a.window, a.sinks, 5);
+    s.span = kv4_span(s.q.pos0, s.q.pos0 + s.q.n - 1, s.q.len, a.window, a.sinks, step_gran(a.cache.page_shift));
     const long long rows = static_cast<long long>(s.q.n) * a.group;
     s.chunks = rows > 0 && rows <= a.step_rows ? kv4_span_chunks(s.span) : 0;
     return s;
@@ -214,49 +253,62 @@ __device__ __forceinline__ void kv4_store_row(const Kv4Attn& a, int first, int r
 }
 
 template <class C, bool BF16>
-__global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_step(const Kv4Attn a) {
+__global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Attn a) {
     constexpr int D = C::D, NT = C::NT, ROWS = C::ROWS, ST = C::ST;
     constexpr int KS = D / 16;   // k-steps of K Q^T
     constexpr int MT = D / 16;   // 16-row tiles of V^T
     extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t* ring = smem;
-    float* merge = reinterpret_cast<float*>(smem);
-    uint2* qfrag = reinterpret_cast<uint2*>(smem + C::UNION);
-    float* sm_m = reinterpret_cast<float*>(smem + C::UNION + C::QFRAG);
+    float* merge = reinterpret_cast<float*>(smem + C::OFF_MERGE);
+    uint2* qfrag = reinterpret_cast<uint2*>(smem + C::OFF_Q);
+    float* sm_m = reinterpret_cast<float*>(smem + C::OFF_ML);
     float* sm_l = sm_m + kStepWarps * ROWS;
-    float* sm_scale = sm_l + kStepWarps * ROWS;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sm_scale + ROWS);
-    long long* sums = reinterpret_cast<long long*>(bars + kStepWarps * ST);  // one per warp, then the result
-    volatile int* abort = reinterpret_cast<volatile int*>(sums + kStepWarps + 2);
+    float* sm_scale = reinterpret_cast<float*>(smem + C::OFF_SCALE);
+    int2* info = reinterpret_cast<int2*>(smem + C::OFF_INFO);  // per stage and warp: first token, flags
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    uint64_t* empty = full + ST;
+    long long* sums = reinterpret_cast<long long*>(smem + C::OFF_SUMS);  // one per warp, then the result
+    volatile int* abort = reinterpret_cast<volatile int*>(sums + kStepThreads / 32 + 2);
+
+    volatile int* failed = abort + 1;  // by a computing warp, before its second barrier of a unit
 
     grid_dep_launch_dependents();  // k_kv4_join waits for this grid's end
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     const int g = lane >> 2, c = lane & 3;
-    uint64_t* bar = bars + warp * ST;
-    if (lane == 0) {
-        for (int i = 0; i < ST; ++i) mbar_init(&bar[i], 1);
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kStepWarps);
+        }
         fence_barrier_init();
+        *abort = 0;
+        *failed = 0;
     }
-    if (tid == 0) *abort = 0;
     __syncthreads();
 
     // This CTA's run of chunks: sequence b, offset `off` in it, `left` chunks.
     int b = 0;
     long long off = 0, left = 0;
-    int my_run = blockIdx.x;
-    if (a.whole) {
-        b = blockIdx.x / a.cache.heads;
+    const int my_run = blockIdx.x;
+    if (a.cluster) {
+        const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
+        b = unit / a.cache.heads;
         const StepSeq s = step_seq(a, b);
-        step_report(a, s);
-        if (s.chunks == 0) return;
-        off = static_cast<long long>(blockIdx.x - b * a.cache.heads) * s.chunks;
-        left = s.chunks;
+        if (tid == 0) step_report(a, s);
+        if (s.chunks == 0) return;  // every CTA of the cluster
+        const int from = static_cast<int>(run_start(s.chunks, a.cluster, rank));
+        off = static_cast<long long>(unit - b * a.cache.heads) * s.chunks + from;
+        left = run_start(s.chunks, a.cluster, rank + 1) - from;
     } else {
-        long long sum = 0;
-        for (int i = tid; i < a.rows.batch; i += blockDim.x) {
+        // The chunks of all sequences and of those before each one: a thread
+        // takes the sequences tid, tid + 384, ...
+        constexpr int kWarps = kStepThreads / 32;
+        long long mine = 0, sum = 0;
+        for (int i = tid; i < a.rows.batch; i += kStepThreads) {
             const StepSeq s = step_seq(a, i);
-            step_report(a, s);
-            sum += s.total(a.cache.heads);
+            if (my_run == 0) step_report(a, s);
+            const long long w = s.total(a.cache.heads);
+            if (i == tid) mine = w;
+            sum += w;
         }
         const long long total = block_sum(sum, sums);
         const int runs = step_runs(a, total);
@@ -265,9 +317,9 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
         left = run_start(total, runs, my_run + 1) - from;
         if (left <= 0) return;
         long long before = 0;
-        for (int b0 = 0; b0 < a.rows.batch; b0 += blockDim.x) {
+        for (int b0 = 0; b0 < a.rows.batch && before <= from; b0 += kStepThreads) {
             const int i = b0 + tid;
-            const long long w = i < a.rows.batch ? step_seq(a, i).total(a.cache.heads) : 0;
+            const long long w = b0 == 0 ? mine : i < a.rows.batch ? step_seq(a, i).total(a.cache.heads) : 0;
             long long upto = w;  // inclusive sum over the CTA's threads
             for (int d = 1; d < 32; d <<= 1) {
                 const long long o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
@@ -277,46 +329,160 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
             if (lane == 31) sums[warp] = upto;
             __syncthreads();
             long long all = 0;
-            for (int k = 0; k < kStepWarps; ++k) {
+            for (int k = 0; k < kWarps; ++k) {
                 if (k < warp) upto += sums[k];
                 all += sums[k];
             }
             const long long lo = before + upto - w;
             if (w > 0 && from >= lo && from < lo + w) {
-                sums[kStepWarps] = i;
-                sums[kStepWarps + 1] = from - lo;
+                sums[kWarps] = i;
+                sums[kWarps + 1] = from - lo;
             }
             before += all;
-            if (before > from) break;
         }
         __syncthreads();
-        b = static_cast<int>(sums[kStepWarps]);
-        off = sums[kStepWarps + 1];
+        b = static_cast<int>(sums[kWarps]);
+        off = sums[kWarps + 1];
     }
 
-    uint32_t used = 0;  // chunks this warp has taken through its ring
-    const float thr = 8.0f;
-    while (left > 0 && b < a.rows.batch) {
+    // Chunk geometry.  A stage holds a tile of 256 tokens as whole chunks; a
+    // chunk is a page's block of this head as it lies in the cache, two of
+    // them for 16-token pages, or 256 tokens of a larger page.
+    const int shift = a.cache.page_shift, gs = step_gran(shift);
+    const uint32_t gran = 1u << gs;
+    const int per_tile = kStepTile >> gs;
+    const uint32_t codes = kv4_codes_bytes(a.cache), scales = kv4_scales_bytes(a.cache);
+    const uint32_t block_tokens = shift == 4 ? 16u : gran;  // contiguous in the stage: Kc, Ks, Vc, Vs
+    const uint32_t at_ks = block_tokens * (D / 2), at_vc = at_ks + block_tokens * (D / 16),
+                   at_vs = at_vc + block_tokens * (D / 2), block_bytes = block_tokens * C::TOKEN_BYTES * 2;
+
+    int stage = 0;
+    uint32_t phase = 0;
+    if (warp >= kStepWarps) {
+        reg_dec<C::REGS_LOAD>();
+        if (warp > kStepWarps) return;
+        // ---- the loading warp: lane i < 16 looks after tokens 16 i .. + 15 of a tile ----
+        const int sub = lane * 16;                       // place in the tile
+        const int entry = sub >> gs;                     // its chunk of the tile
+        const bool leads = lane < 16 && (sub & static_cast<int>(block_tokens - 1)) == 0;  // first of a block
+        uint32_t filled = 0;
+        while (left > 0 && b < a.rows.batch) {
+            const StepSeq s = step_seq(a, b);
+            if (off >= s.total(a.cache.heads)) {
+                off -= s.total(a.cache.heads);
+                ++b;
+                continue;
+            }
+            const int head = static_cast<int>(off / s.chunks);
+            const int c0 = static_cast<int>(off - static_cast<long long>(head) * s.chunks);
+            const int c1 = left < s.chunks - c0 ? c0 + static_cast<int>(left) : s.chunks;
+            left -= c1 - c0;
+            off += c1 - c0;
+            if (lane == 0 && s.q.bad) atomicOr(&g_tb_device_error, kErrPage);
+            const int* table = a.rows.table + static_cast<size_t>(b) * a.rows.width;
+            const uint8_t* blocks = a.cache.data + static_cast<size_t>(head) * kv4_head_bytes(a.cache);
+            // A chunk at token tok0 is open (every row sees all of it) if it ends
+            // by `open_end` and starts by `open_low` or ends in the sinks.
+            const int last_pos = s.q.pos0 + s.q.n - 1;
+            const int open_end = min(s.q.pos0 + 1, s.q.len);
+            const int open_low = a.window > 0 && last_pos >= a.window ? last_pos - a.window + 1 : 0;
+            // Token and page number of this lane's granule of the tile at chunk q.
+            auto look = [&](int q, int& tok, int& page) {
+                tok = -1;
+                page = -1;
+                if (lane < 16 && q + entry < c1) {
+                    tok = (kv4_span_chunk(s.span, q + entry) << gs) + (sub & static_cast<int>(gran - 1));
+                    if (tok < s.q.len) page = table[tok >> shift];
+                }
+            };
+            int tok, page;
+            look(c0, tok, page);
+            for (int q = c0; q < c1; q += per_tile) {
+                if (!__all_sync(0xFFFFFFFFu, filled < ST || mbar_wait(&empty[stage], phase ^ 1u, abort))) break;
+                const bool inside = tok >= 0 && tok < s.q.len;
+                const bool ok = inside && kv4_page_ok(a.cache, page);
+                if (inside && !ok) atomicOr(&g_tb_device_error, kErrPage);
+                const uint32_t have = __ballot_sync(0xFFFFFFFFu, ok);
+                const uint32_t copies = __ballot_sync(0xFFFFFFFFu, ok && leads);
+                if (lane < 16 && (lane & 1) == 0) {
+                    const uint32_t two = (have >> lane) & 3u;
+                    const bool open = two == 3u && tok + kStepChunk <= open_end &&
+                                      (tok >= open_low || tok + kStepChunk <= a.sinks);
+                    info[stage * kStepWarps + lane / 2] = make_int2(tok, static_cast<int>(two | (open ? 4u : 0u)));
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&full[stage], __popc(copies) * block_bytes);
+                __syncwarp();
+                uint8_t* dst = smem + stage * C::STAGE + (sub / static_cast<int>(block_tokens)) * block_bytes;
+                if (shift <= 8) {
+                    if (ok && leads)
+                        bulk_load(dst, blocks + static_cast<unsigned long long>(static_cast<uint32_t>(page)) * a.cache.page_stride,
+                                  block_bytes, &full[stage]);
+                } else if (ok && leads) {  // lane 0: a tile of a larger page, part by part
+                    const uint32_t place = static_cast<uint32_t>(tok) & ((1u << shift) - 1u);
+                    const uint8_t* src =
+                        blocks + static_cast<unsigned long long>(static_cast<uint32_t>(page)) * a.cache.page_stride;
+                    bulk_load(dst, src + place * (D / 2), at_ks, &full[stage]);
+                    bulk_load(dst + at_ks, src + codes + place * (D / 16), at_vc - at_ks, &full[stage]);
+                    src += codes + scales;
+                    bulk_load(dst + at_vc, src + place * (D / 2), at_ks, &full[stage]);
+                    bulk_load(dst + at_vs, src + codes + place * (D / 16), at_vc - at_ks, &full[stage]);
+                }
+                __syncwarp();
+                ++filled;
+                if (++stage == ST) stage = 0, phase ^= 1u;
+                if (q + per_tile < c1) look(q + per_tile, tok, page);
+            }
+            if (__any_sync(0xFFFFFFFFu, *abort)) break;
+        }
+        if (*abort)  // copies in flight end before the CTA does
+            for (int i = 0; i < ST && filled > 0; ++i, --filled) {
+                if (--stage < 0) stage = ST - 1, phase ^= 1u;
+                mbar_wait_drain(&full[stage], phase);
+            }
+        return;
+    }
+
+    // ---- the computing warps: 32 tokens of a tile each ------------------------------------
+    reg_inc<C::REGS_COMPUTE>();
+    // Where the warp's tokens lie in a stage; tokens 16..31 follow 16 places on, or in the next block.
+    const uint32_t in_block = (warp * kStepChunk) & (block_tokens - 1u);
+    const uint32_t block0 = (warp * kStepChunk) / block_tokens * block_bytes;
+    const uint32_t half_step = shift == 4 ? block_bytes : 16u * (D / 2), half_step_s = shift == 4 ? block_bytes : 16u * (D / 16);
+    const int tg = g ^ ((g >> 1) & 1);
+    // Row g of a 16-token tile is token g ^ (g >> 1 & 1): neighbouring lanes of
+    // the loads of K and of V then fall into different banks.
+    const uint32_t k_codes = block0 + in_block * (D / 2) + tg * (D / 2) + c * (D / 8);
+    const uint32_t k_scales = block0 + at_ks + in_block * (D / 16) + tg * (D / 16) + c * (D / 64);
+    const uint32_t ta = static_cast<uint32_t>((2 * c) ^ (c & 1));  // V: tokens ta, ta ^ 1, and 8 on
+    const uint32_t v_codes = block0 + at_vc + (in_block + ta) * (D / 2) + g * (D / 16);
+    const uint32_t v_scales = block0 + at_vs + (in_block + ta) * (D / 16) + (g * (D / 16)) / 8;
+    const int v_pair = ta & 1u ? -1 : 1;  // from token ta to ta ^ 1
+
+    // A CTA of a cluster has one pass, with or without chunks.
+    for (bool once = a.cluster != 0; (once || left > 0) && b < a.rows.batch; once = false) {
         const StepSeq s = step_seq(a, b);
-        if (off >= s.total(a.cache.heads)) {
+        if (off >= s.total(a.cache.heads) && left > 0) {
             off -= s.total(a.cache.heads);
             ++b;
             continue;
         }
-        const int head = static_cast<int>(off / s.chunks);
+        const int head = a.cluster ? blockIdx.x / a.cluster - b * a.cache.heads : static_cast<int>(off / s.chunks);
         const int c0 = static_cast<int>(off - static_cast<long long>(head) * s.chunks);
         const int c1 = left < s.chunks - c0 ? c0 + static_cast<int>(left) : s.chunks;
         const int row_count = s.q.n * a.group;  // at most ROWS
         left -= c1 - c0;
         off += c1 - c0;
-        if (tid == 0 && s.q.bad) atomicOr(&g_tb_device_error, kErrPage);
 
         // Queries in fragment order: lane (g, c) of k-step ks holds, for row
         // g, the values d = (D/4) c + 4 ks .. + 3, each pair swapped as the
         // converter leaves a byte's two codes.
         for (int r = warp; r < ROWS; r += kStepWarps) {
             uint2 v = make_uint2(0u, 0u);
-            float scale = a.scale_log2;
+            // The factor is taken positive, its sign into q: the largest product
+            // is the largest score.  Not zero, which would make NaN of -inf.
+            float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);
+            const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
             if (r < row_count) {
                 const int i = r / a.group;
                 const long long at = (s.q.first + i) * a.q_stride +
@@ -330,11 +496,13 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                     e = __reduce_max_sync(0xFFFFFFFFu, e);
                     const int k = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = k > 120 ? 120 : k, k2 = k - k1;
                     const float up = exp2i(k1), up2 = exp2i(k2);
-                    scale = (scale * exp2i(-k1)) * exp2i(-k2);
+                    scale = fmaxf((scale * exp2i(-k1)) * exp2i(-k2), 1e-37f);
                     v.x = pack_half2(__uint_as_float(v.x << 16) * up * up2, __uint_as_float(v.x & 0xFFFF0000u) * up * up2);
                     v.y = pack_half2(__uint_as_float(v.y << 16) * up * up2, __uint_as_float(v.y & 0xFFFF0000u) * up * up2);
                 }
             }
+            v.x ^= sign;
+            v.y ^= sign;
             if (lane < D / 4) {
                 const int ks = lane % KS, cc = lane / KS;
                 qfrag[((r / 8) * KS + ks) * 32 + (r % 8) * 4 + cc] =
@@ -342,7 +510,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
             }
             if (lane == 0) sm_scale[r] = scale;
         }
-        __syncthreads();
+        named_bar_sync(1, 32 * kStepWarps);
 
         float sf[NT][2];  // score -> log2 units, of rows 8 nt + 2c, + 1
         float m[NT][2], l[NT][2];
@@ -352,7 +520,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 sf[nt][e] = sm_scale[8 * nt + 2 * c + e];
-                m[nt][e] = -INFINITY;
+                m[nt][e] = kNoMax;
                 l[nt][e] = 0.0f;
             }
 #pragma unroll
@@ -362,154 +530,85 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[mt][nt][e] = 0.0f;
 
-        // Chunk geometry: pages of 16 and of 32 tokens come with all four
-        // parts of a page's head block in one copy; larger pages part by part.
-        const int shift = a.cache.page_shift;
-        const uint32_t codes = kv4_codes_bytes(a.cache), scales = kv4_scales_bytes(a.cache);
-        const uint32_t unit_tokens = shift == 4 ? 16u : 32u;
-        const uint32_t half_step = shift == 4 ? 16u * C::TOKEN_BYTES * 2 : 16u * (D / 2);  // codes of tokens 16..31
-        const uint32_t half_step_s = shift == 4 ? half_step : 16u * (D / 16);              // scales of tokens 16..31
-        const uint32_t at_ks = unit_tokens * (D / 2), at_vc = at_ks + unit_tokens * (D / 16),
-                       at_vs = at_vc + unit_tokens * (D / 2);
-        const int* table = a.rows.table + static_cast<size_t>(b) * a.rows.width;
-        const int first_pos = s.q.pos0, last_pos = s.q.pos0 + s.q.n - 1;  // of the rows
-
-        // Page numbers of a chunk: two for 16-token pages.
-        auto look = [&](int q, int& p0, int& p1) {
-            p0 = p1 = -1;
-            if (q >= c1) return;
-            const int tok = kv4_span_chunk(s.span, q) * kStepChunk;
-            if (tok < s.q.len) p0 = table[tok >> shift];
-            if (shift == 4 && tok + 16 < s.q.len) p1 = table[(tok >> shift) + 1];
-        };
-        // Start the copies of chunk q into `stage`; returns which halves hold tokens.
-        auto issue = [&](int q, int p0, int p1, int stage) -> uint32_t {
-            const int tok = kv4_span_chunk(s.span, q) * kStepChunk;
-            uint32_t have = 0;
-            const bool ok0 = tok < s.q.len && kv4_page_ok(a.cache, p0);
-            const bool ok1 = shift == 4 ? tok + 16 < s.q.len && kv4_page_ok(a.cache, p1) : ok0;
-            have = (ok0 ? 1u : 0u) | (ok1 ? 2u : 0u);
-            if (lane == 0) {
-                uint8_t* dst = ring + (warp * ST + stage) * C::STAGE;
-                if ((tok < s.q.len && !ok0) || (shift == 4 && tok + 16 < s.q.len && !ok1))
-                    atomicOr(&g_tb_device_error, kErrPage);
-                const uint32_t bytes = shift == 4 ? (ok0 + ok1) * (C::STAGE / 2) : ok0 ? C::STAGE : 0u;
-                mbar_arrive_expect_tx(&bar[stage], bytes);
-                if (shift <= 5) {
-                    if (ok0)
-                        bulk_load(dst, a.cache.data + kv4_block_offset(a.cache, p0, head),
-                                  shift == 4 ? C::STAGE / 2 : C::STAGE, &bar[stage]);
-                    if (shift == 4 && ok1)
-                        bulk_load(dst + C::STAGE / 2, a.cache.data + kv4_block_offset(a.cache, p1, head), C::STAGE / 2,
-                                  &bar[stage]);
-                } else if (ok0) {
-                    const uint32_t place = static_cast<uint32_t>(tok) & ((1u << shift) - 1u);
-                    const uint8_t* src = a.cache.data + kv4_block_offset(a.cache, p0, head);
-                    bulk_load(dst, src + place * (D / 2), kStepChunk * (D / 2), &bar[stage]);
-                    bulk_load(dst + at_ks, src + codes + place * (D / 16), kStepChunk * (D / 16), &bar[stage]);
-                    src += codes + scales;
-                    bulk_load(dst + at_vc, src + place * (D / 2), kStepChunk * (D / 2), &bar[stage]);
-                    bulk_load(dst + at_vs, src + codes + place * (D / 16), kStepChunk * (D / 16), &bar[stage]);
-                }
-            }
-            return have;
-        };
-
-        uint32_t halves = 0;  // which halves of the chunks in flight hold tokens: two bits a stage
-        int next = c0 + warp, p0, p1;
-        const int mine = next < c1 ? (c1 - next + kStepWarps - 1) / kStepWarps : 0;
-#pragma unroll
-        for (int i = 0; i < ST; ++i) {
-            if (i < mine) {
-                look(next, p0, p1);
-                const int stage = (used + i) % ST;
-                halves = (halves & ~(3u << (2 * stage))) | (issue(next, p0, p1, stage) << (2 * stage));
-                next += kStepWarps;
-            }
-        }
-        look(next, p0, p1);
-
-        for (int it = 0; it < mine; ++it) {
-            const int stage = used % ST;
-            const uint32_t parity = (used / ST) & 1u;
-            ++used;
-            const int tok0 = kv4_span_chunk(s.span, c0 + warp + it * kStepWarps) * kStepChunk;
-            if (!mbar_wait(&bar[stage], parity, abort)) {
-                // Let the copies in flight end before the ring is given up.
-                const int flying = min(ST, mine - it);
-                for (int i = 0; i < flying; ++i)
-                    mbar_wait_drain(&bar[(used - 1 + i) % ST], ((used - 1 + i) / ST) & 1u);
+        for (int q = c0; q < c1; q += per_tile) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[stage], phase, abort))) {
+                *failed = 1;
                 break;
             }
-            const uint32_t base = smem_addr(ring + (warp * ST + stage) * C::STAGE);
-            const uint32_t have = (halves >> (2 * stage)) & 3u;
-            // Every row sees the whole chunk, and all of it is there.
-            const bool open = have == 3u && tok0 + kStepChunk - 1 <= first_pos &&
-                              tok0 + kStepChunk <= s.q.len &&
-                              (a.window <= 0 || last_pos - tok0 < a.window || tok0 + kStepChunk <= a.sinks);
+            const int2 what = info[stage * kStepWarps + warp];
+            const int tok0 = what.x;
+            const uint32_t have = what.y & 3u;
+            const bool open = what.y & 4;
+            const uint32_t base = smem_addr(smem) + stage * C::STAGE;
+            uint64_t* done = &empty[stage];
+            if (++stage == ST) stage = 0, phase ^= 1u;
+            if (have == 0u) {  // nothing of this warp's share exists
+                __syncwarp();
+                if (lane == 0) mbar_arrive(done);
+                continue;
+            }
 
+            // S^T = K Q^T of two times 16 tokens.
             float sc[2][NT][4];
+            {
+                uint32_t ka[2][D / 32], kc[2][D / 32];  // codes of rows g and g + 8
+                uint32_t sa[2][D / 64], sd[2][D / 64];  // their scales, doubled
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t kb = base + k_codes + t * half_step, sb = base + k_scales + t * half_step_s;
+                    if constexpr (D == 128) {
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(ka[t][0]), "=r"(ka[t][1]), "=r"(ka[t][2]), "=r"(ka[t][3]) : "r"(kb));
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(kc[t][0]), "=r"(kc[t][1]), "=r"(kc[t][2]), "=r"(kc[t][3])
+                                     : "r"(kb + 8 * (D / 2)));
+                        uint16_t x, y;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(sb));
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(sb + 8 * (D / 16)));
+                        const uint32_t xx = cvt_e4m3x2(x), yy = cvt_e4m3x2(y);
+                        sa[t][0] = prmt(xx, 0u, 0x1010u); sa[t][1] = prmt(xx, 0u, 0x3232u);
+                        sd[t][0] = prmt(yy, 0u, 0x1010u); sd[t][1] = prmt(yy, 0u, 0x3232u);
+                    } else {
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(ka[t][0]), "=r"(ka[t][1]) : "r"(kb));
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                                     : "=r"(kc[t][0]), "=r"(kc[t][1]) : "r"(kb + 8 * (D / 2)));
+                        uint32_t x, y;
+                        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(sb));
+                        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(y) : "r"(sb + 8 * (D / 16)));
+                        sa[t][0] = cvt_e4m3x2(static_cast<uint16_t>(x | (x << 8)));
+                        sd[t][0] = cvt_e4m3x2(static_cast<uint16_t>(y | (y << 8)));
+                    }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[t][nt][e] = 0.0f;
-                // Row g of the tile is token g ^ (g >> 1 & 1): neighbouring
-                // lanes of the loads below then fall into different banks.
-                const uint32_t tok = static_cast<uint32_t>(g ^ ((g >> 1) & 1));
-                const uint32_t kb = base + t * half_step + tok * (D / 2) + c * (D / 8);
-                const uint32_t sb = base + at_ks + t * half_step_s + tok * (D / 16) + c * (D / 64);
-                uint32_t ka[D / 32], kc[D / 32];  // codes of tokens g and g + 8
-                uint32_t sa[D / 64], sd[D / 64];  // their scales, doubled
-                if constexpr (D == 128) {
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(ka[0]), "=r"(ka[1]), "=r"(ka[2]), "=r"(ka[3]) : "r"(kb));
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(kc[0]), "=r"(kc[1]), "=r"(kc[2]), "=r"(kc[3]) : "r"(kb + 8 * (D / 2)));
-                    uint16_t x, y;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(sb));
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(sb + 8 * (D / 16)));
-                    const uint32_t xx = cvt_e4m3x2(x), yy = cvt_e4m3x2(y);
-                    sa[0] = prmt(xx, 0u, 0x1010u); sa[1] = prmt(xx, 0u, 0x3232u);
-                    sd[0] = prmt(yy, 0u, 0x1010u); sd[1] = prmt(yy, 0u, 0x3232u);
-                } else {
-                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(ka[0]), "=r"(ka[1]) : "r"(kb));
-                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(kc[0]), "=r"(kc[1]) : "r"(kb + 8 * (D / 2)));
-                    uint32_t x, y;
-                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(sb));
-                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(y) : "r"(sb + 8 * (D / 16)));
-                    sa[0] = cvt_e4m3x2(static_cast<uint16_t>(x | (x << 8)));
-                    sd[0] = cvt_e4m3x2(static_cast<uint16_t>(y | (y << 8)));
+                        for (int e = 0; e < 4; ++e) sc[t][nt][e] = 0.0f;
                 }
 #pragma unroll
                 for (int w = 0; w < D / 32; ++w) {
-                    uint32_t fa[4], fc[4];
-                    cvt_e2m1x2_x4(ka[w], fa);
-                    cvt_e2m1x2_x4(kc[w], fc);
+                    uint32_t fa[2][4], fc[2][4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        fa[j] = hmul2(fa[j], sa[w / 2]);
-                        fc[j] = hmul2(fc[j], sd[w / 2]);
+                    for (int t = 0; t < 2; ++t) {
+                        cvt_e2m1x2_x4(ka[t][w], fa[t]);
+                        cvt_e2m1x2_x4(kc[t][w], fc[t]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            fa[t][j] = hmul2(fa[t][j], sa[t][w / 2]);
+                            fc[t][j] = hmul2(fc[t][j], sd[t][w / 2]);
+                        }
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             const uint2 qf = qfrag[(nt * KS + 2 * w + h) * 32 + lane];
-                            mma_16816(sc[t][nt], fa[2 * h], fc[2 * h], fa[2 * h + 1], fc[2 * h + 1], qf.x, qf.y);
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                mma_16816(sc[t][nt], fa[t][2 * h], fc[t][2 * h], fa[t][2 * h + 1], fc[t][2 * h + 1], qf.x,
+                                          qf.y);
                         }
                 }
             }
 
-            // Scores in log2 units; hidden ones are -inf.
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[t][nt][e] *= sf[nt][e & 1];
-            const int tg = g ^ ((g >> 1) & 1);
             if (!open) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -526,67 +625,63 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                             }
                     }
             }
+            // In log2 units a score is s f - m; a row whose largest passes 2^8 moves its m.
             bool past = false;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) past |= sc[t][nt][e] > m[nt][e & 1] + thr;
+                for (int e = 0; e < 2; ++e)
+                    past |= fmaf(fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2])),
+                                 sf[nt][e], -m[nt][e]) > 8.0f;
             if (__any_sync(0xFFFFFFFFu, past)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float x = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
+                        float y = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
 #pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
-                        x = fmaxf(x, m[nt][e]);
-                        const float f = x == -INFINITY ? 1.0f : ex2(m[nt][e] - x);
-                        m[nt][e] = x;
-                        l[nt][e] *= f;
+                        for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xFFFFFFFFu, y, d));
+                        y = fmaxf(y * sf[nt][e], m[nt][e]);
+                        const float r = ex2(m[nt][e] - y);
+                        m[nt][e] = y;
+                        l[nt][e] *= r;
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            o[mt][nt][e] *= f;
-                            o[mt][nt][e + 2] *= f;
+                            o[mt][nt][e] *= r;
+                            o[mt][nt][e + 2] *= r;
                         }
                     }
             }
             uint32_t pf[2][NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0];
-                const float m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    float x[4];
+                    float p[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = ex2(sc[t][nt][e] - (e & 1 ? m1 : m0));
-                    l[nt][0] += x[0] + x[2];
-                    l[nt][1] += x[1] + x[3];
-                    pf[t][nt][0] = movmatrix(pack_half2(x[0], x[1]));
-                    pf[t][nt][1] = movmatrix(pack_half2(x[2], x[3]));
+                    for (int e = 0; e < 4; ++e) p[e] = ex2(fmaf(sc[t][nt][e], sf[nt][e & 1], -m[nt][e & 1]));
+                    l[nt][0] += p[0] + p[2];
+                    l[nt][1] += p[1] + p[3];
+                    pf[t][nt][0] = movmatrix(pack_half2(p[0], p[1]));
+                    pf[t][nt][1] = movmatrix(pack_half2(p[2], p[3]));
                 }
-            }
 
             // O^T += V^T P^T.  The lane's tokens 2c, 2c+1, 2c+8, 2c+9 of the
             // 16, and its D/8 values d of each.
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const uint32_t ta = static_cast<uint32_t>((2 * c) ^ (c & 1)), tb2 = ta ^ 1u;
-                const uint32_t vb = base + at_vc + t * half_step + g * (D / 16);
-                const uint32_t sb = base + at_vs + t * half_step_s + (g * (D / 16)) / 8;
+                const uint32_t vb = base + v_codes + t * half_step, sb = base + v_scales + t * half_step_s;
                 constexpr int VW = D / 64;  // words of a token
                 uint32_t v[4][VW], sv[4];
-                const uint32_t tk[4] = {ta, tb2, ta + 8, tb2 + 8};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
+                    const uint32_t at = vb + ((k & 1) * v_pair + (k >> 1) * 8) * (D / 2);
                     if constexpr (VW == 2)
-                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                                     : "=r"(v[k][0]), "=r"(v[k][VW - 1]) : "r"(vb + tk[k] * (D / 2)));
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[k][0]), "=r"(v[k][VW - 1]) : "r"(at));
                     else
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[k][0]) : "r"(vb + tk[k] * (D / 2)));
-                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(sv[k]) : "r"(sb + tk[k] * (D / 16)));
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[k][0]) : "r"(at));
+                    asm volatile("ld.shared.u8 %0, [%1];"
+                                 : "=r"(sv[k]) : "r"(sb + ((k & 1) * v_pair + (k >> 1) * 8) * (D / 16)));
                 }
                 if (!open) {
                     // A token that a row does not see adds nothing to it, NaN
@@ -595,7 +690,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                     uint32_t nan = 0;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int tok = tok0 + 16 * t + static_cast<int>(tk[k]);
+                        const int tok = tok0 + 16 * t + static_cast<int>(ta) + (k & 1) * v_pair + 8 * (k >> 1);
                         const bool there = ((have >> t) & 1u) && tok < s.q.len;
                         if (!there) sv[k] = 0u;
                         if ((sv[k] & 0x7Fu) == 0x7Fu) {
@@ -644,11 +739,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
             }
 
             __syncwarp();
-            if (it + ST < mine) {
-                halves = (halves & ~(3u << (2 * stage))) | (issue(next, p0, p1, stage) << (2 * stage));
-                next += kStepWarps;
-                look(next, p0, p1);
-            }
+            if (lane == 0) mbar_arrive(done);
         }
 
         // Merge the warps: m and l first, then o scaled to the common maximum.
@@ -663,16 +754,16 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                     sm_l[warp * ROWS + 8 * nt + 2 * c + e] = l[nt][e];
                 }
             }
-        __syncthreads();  // also: nobody reads the ring any more
+        named_bar_sync(1, 32 * kStepWarps);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = 8 * nt + 2 * c + e;
-                float top = -INFINITY;
+                float top = kNoMax;
 #pragma unroll
                 for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sm_m[w * ROWS + r]);
-                const float f = m[nt][e] == -INFINITY ? 0.0f : ex2(m[nt][e] - top);
+                const float f = ex2(m[nt][e] - top);
                 float* at = merge + (warp * ROWS + r) * (D + 4) + g * (D / 8);
 #pragma unroll
                 for (int k = 0; k < MT / 2; ++k) {
@@ -681,24 +772,28 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                                     o[2 * k + 1][nt][e + 2] * f);
                 }
             }
-        __syncthreads();
-        const bool partial = !(c0 == 0 && c1 == s.chunks);
+        named_bar_sync(1, 32 * kStepWarps);
+        if (*failed && a.cluster == 0) return;  // all of them
+        const bool partial = !(c0 == 0 && c1 == s.chunks) && a.cluster == 0;
         float* slot = partial ? step_slot<C>(a.ws, my_run, c0 == 0 ? 1 : 0) : nullptr;
         for (int x = tid; x < row_count * (D / 4); x += kStepWarps * 32) {
             const int r = x / (D / 4), d = 4 * (x % (D / 4));
-            float top = -INFINITY;
+            float top = kNoMax;
 #pragma unroll
             for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sm_m[w * ROWS + r]);
             float sum = 0.0f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kStepWarps; ++w) {
-                const float mw = sm_m[w * ROWS + r];
-                sum += sm_l[w * ROWS + r] * (mw == -INFINITY ? 0.0f : ex2(mw - top));  // NaN stays NaN
+                sum += sm_l[w * ROWS + r] * ex2(sm_m[w * ROWS + r] - top);
                 const float4 u = *reinterpret_cast<const float4*>(merge + (w * ROWS + r) * (D + 4) + d);
                 v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
             }
-            if (partial) {
+            if (a.cluster > 1) {  // into the ring, which is idle: o [row][D + 4] with m and l behind
+                float* part = reinterpret_cast<float*>(smem) + r * (D + 4);
+                *reinterpret_cast<float4*>(part + d) = v;
+                if (d == 0) *reinterpret_cast<float2*>(part + D) = make_float2(top, sum);
+            } else if (partial) {
                 *reinterpret_cast<float4*>(slot + r * D + d) = v;
                 if (d == 0) {
                     slot[ROWS * D + r] = top;
@@ -708,23 +803,43 @@ __global__ void __launch_bounds__(kStepWarps * 32, C::NT == 1 ? 2 : 1) k_kv4_ste
                 kv4_store_row<BF16, D>(a, s.q.first, r, head, d, v, top, sum);
             }
         }
-        // The merge area becomes the ring again: generic accesses first.
-        fence_proxy_async_smem();
-        __syncthreads();
-        if (*abort) return;
+        if (a.cluster > 1) {
+            // The CTAs of the cluster join their results through distributed
+            // shared memory, each some of the values.
+            __syncwarp();
+            cluster_sync();
+            const int rank = static_cast<int>(cluster_ctarank());
+            for (int x = tid * a.cluster + rank; x < row_count * (D / 4); x += 32 * kStepWarps * a.cluster) {
+                const int r = x / (D / 4), d = 4 * (x % (D / 4));
+                float top = kNoMax, l = 0.0f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                for (int k = 0; k < a.cluster; ++k) {
+                    const uint32_t part = cluster_addr(smem, k) + r * (D + 4) * 4;
+                    const float4 u = ld_cluster4(part + 4 * d), ml = ld_cluster4(part + 4 * D);
+                    kv4_merge(top, l, v, ml.x, ml.y, u);
+                }
+                kv4_store_row<BF16, D>(a, s.q.first, r, head, d, v, top, l);
+            }
+            __syncwarp();
+            cluster_sync();  // nobody leaves while its part is read
+        }
     }
 }
 
-// Joins the partial results of the units that more than one run shares, in the
-// order of the runs.  One CTA per unit that may exist.
+// Joins the partial results of the units that more than one run shares, in a
+// fixed order: four threads of a row's float4 take every fourth run each and
+// are joined in shared memory.  A CTA has 256 / D rows of a unit (blockIdx.y).
 template <class C, bool BF16>
 __global__ void __launch_bounds__(256) k_kv4_join(const Kv4Attn a) {
-    constexpr int D = C::D, ROWS = C::ROWS;
+    constexpr int D = C::D, ROWS = C::ROWS, LANES = D / 4;
     __shared__ long long sums[8];
-    grid_dep_wait();
+    __shared__ float4 part_v[4][256 / 4];
+    __shared__ float2 part_ml[4][256 / 4];
     const int b = blockIdx.x / a.cache.heads, head = blockIdx.x - b * a.cache.heads;
     const StepSeq s = step_seq(a, b);
-    if (s.chunks == 0) return;
+    const int row0 = blockIdx.y * (64 / LANES);
+    if (s.chunks == 0 || row0 >= s.q.n * a.group) return;
     long long sum = 0, sum_before = 0;
     for (int i = threadIdx.x; i < a.rows.batch; i += blockDim.x) {
         const long long w = step_seq(a, i).total(a.cache.heads);
@@ -736,16 +851,26 @@ __global__ void __launch_bounds__(256) k_kv4_join(const Kv4Attn a) {
     const long long u0 = before + static_cast<long long>(head) * s.chunks, u1 = u0 + s.chunks;
     const int r0 = static_cast<int>(((u0 + 1) * runs - 1) / total), r1 = static_cast<int>((u1 * runs - 1) / total);
     if (r0 == r1) return;  // one run had all of it
-    const int row_count = s.q.n * a.group;
-    for (int x = threadIdx.x; x < row_count * (D / 4); x += blockDim.x) {
-        const int r = x / (D / 4), d = 4 * (x % (D / 4));
-        float top = -INFINITY, l = 0.0f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = r0; i <= r1; ++i) {
+    grid_dep_wait();       // all above is the caller's; the partial results are the step kernel's
+    const int quarter = threadIdx.x / 64, item = threadIdx.x % 64;
+    const int r = row0 + item / LANES, d = 4 * (item % LANES);
+    const bool valid = r < s.q.n * a.group;
+    float top = kNoMax, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (valid) {
+#pragma unroll 4
+        for (int i = r0 + quarter; i <= r1; i += 4) {
             const float* slot = step_slot<C>(a.ws, i, i == r0 ? 1 : 0);
             kv4_merge(top, l, v, slot[ROWS * D + r], slot[ROWS * D + ROWS + r],
                       *reinterpret_cast<const float4*>(slot + r * D + d));
         }
+    }
+    part_v[quarter][item] = v;
+    part_ml[quarter][item] = make_float2(top, l);
+    __syncthreads();
+    if (quarter == 0 && valid) {
+#pragma unroll
+        for (int k = 1; k < 4; ++k) kv4_merge(top, l, v, part_ml[k][item].x, part_ml[k][item].y, part_v[k][item]);
         kv4_store_row<BF16, D>(a, s.q.first, r, head, d, v, top, l);
     }
 }

@@ -12,6 +12,7 @@ from gpu_util import to_dev
 
 pytestmark = pytest.mark.gpu
 
+LONG = 10 ** 6  # a max_len for which sequences are shared by runs of chunks
 EPS = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}  # half a step
 
 
@@ -141,10 +142,12 @@ class Batch:
 
     def run(self, q_heads, scale=None, std=1.0, **kw):
         scale = self.host.dim ** -0.5 if scale is None else scale
+        """Both ways of sharing a sequence: short (clusters) and long (runs of
+        chunks), chosen by max_len."""
         q, dense = self.queries(q_heads, std)
-        out, lse = self.attend(q, q_heads, scale, **kw)
-        self.check(out, lse, dense, q_heads, scale, kw.get("window", 0), kw.get("sinks", 0))
-        return out, lse
+        for max_len in (kw.pop("max_len", None), LONG):
+            out, lse = self.attend(q, q_heads, scale, max_len=max_len, **kw)
+            self.check(out, lse, dense, q_heads, scale, kw.get("window", 0), kw.get("sinks", 0))
 
 
 # ---- append ------------------------------------------------------------------------------
@@ -346,7 +349,7 @@ def test_step_split(tb, cuda, typ, dim, page):
     lens = [2600, 1, 40, 0, 1500, 1025]
     bt = Batch(tb, cuda, lens, [1, 1, 1, 0, 1, 1], page=page, heads=2, dim=dim, typ=typ, seed=page)
     bt.fill_fast()
-    assert tb.kv4_attention_workspace(bt.cache, bt.rows, 8, 1, 2600) > 0
+    assert tb.kv4_attention_workspace(bt.cache, bt.rows, 8, 1, LONG) > 0
     bt.run(8)
 
 
@@ -421,8 +424,9 @@ def test_rising_scores(tb, cuda):
     bt.upload()
     q, dense = bt.queries(4)
     q.abs_()
-    out, lse = bt.attend(q, 4, 1.0)
-    bt.check(out, lse, q, 4, 1.0)
+    for max_len in (None, LONG):
+        out, lse = bt.attend(q, 4, 1.0, max_len=max_len)
+        bt.check(out, lse, q, 4, 1.0)
 
 
 @pytest.mark.parametrize("magnitude", [2.0 ** 100, 2.0 ** 15, 2.0 ** -60, 2.0 ** -120])
@@ -439,15 +443,16 @@ def test_bf16_queries_outside_fp16(tb, cuda, magnitude):
         bt.check(out, lse, q, 4, float(np.float32(scale)))
 
 
+@pytest.mark.parametrize("max_len", [None, LONG])
 @pytest.mark.parametrize("n", [1, 3, 40])
-def test_what_lies_behind_a_sequence_is_not_seen(tb, cuda, n):
+def test_what_lies_behind_a_sequence_is_not_seen(tb, cuda, max_len, n):
     """NaN scales behind the sequences' ends, in unused pages and in unused
     table entries change nothing."""
     lens = [n + 5, 100, 1203]
     bt = Batch(tb, cuda, lens, [n] * 3, page=64, heads=2, dim=128, seed=31)
     bt.fill_fast()
     q, _ = bt.queries(4)
-    first = [x.clone() for x in bt.attend(q, 4, 0.1)]
+    first = [x.clone() for x in bt.attend(q, 4, 0.1, max_len=max_len)]
     used = {(int(bt.table[b, p // 64]), p % 64) for b in range(3) for p in range(lens[b])}
     for page in range(bt.host.pages):
         for place in range(64):
@@ -457,14 +462,15 @@ def test_what_lies_behind_a_sequence_is_not_seen(tb, cuda, n):
                         cs, ss = bt.host.parts(page, h, place, v)
                         bt.host.data[page, ss] = 0x7F + 0x80 * (place & 1)
     bt.upload()
-    again = bt.attend(q, 4, 0.1)
+    again = bt.attend(q, 4, 0.1, max_len=max_len)
     assert cuda.equal(first[0], again[0]) and cuda.equal(first[1], again[1])
     bt.check(*again, q, 4, 0.1)
 
 
+@pytest.mark.parametrize("max_len", [None, LONG])
 @pytest.mark.parametrize("where", ["k", "v"])
 @pytest.mark.parametrize("n", [1, 3, 40])
-def test_nan_tokens_reach_the_rows_that_see_them(tb, cuda, where, n):
+def test_nan_tokens_reach_the_rows_that_see_them(tb, cuda, max_len, where, n):
     """A cached NaN block is seen or hidden like any other token."""
     window, sinks = 50, 2
     lens = [400, 1300]
@@ -478,7 +484,7 @@ def test_nan_tokens_reach_the_rows_that_see_them(tb, cuda, where, n):
             bt.host.data[page, ss.start + 2] = 0x7F  # values 32..47
     bt.upload()
     q, _ = bt.queries(2)
-    out, lse = bt.attend(q, 2, 0.1, window=window, sinks=sinks)
+    out, lse = bt.attend(q, 2, 0.1, window=window, sinks=sinks, max_len=max_len)
     o = out.float().cpu().numpy().reshape(-1, 2, 128)
     for b in range(2):
         for i in range(n):
@@ -499,26 +505,28 @@ def test_nan_tokens_reach_the_rows_that_see_them(tb, cuda, where, n):
             cs, ss = bt.host.parts(page, 0, place, where == "v")
             bt.host.data[page, ss.start + 2] = 0x30
     bt.upload()
-    clean = bt.attend(q, 2, 0.1, window=window, sinks=sinks)[0].float().cpu().numpy().reshape(-1, 2, 128)
+    clean = bt.attend(q, 2, 0.1, window=window, sinks=sinks, max_len=max_len)[0].float().cpu().numpy().reshape(-1, 2, 128)
     np.testing.assert_array_equal(o[ok], clean[ok])
 
 
+@pytest.mark.parametrize("max_len", [None, LONG])
 @pytest.mark.parametrize("n", [1, 40])
-def test_nan_queries_stay_in_their_rows(tb, cuda, n):
+def test_nan_queries_stay_in_their_rows(tb, cuda, max_len, n):
     bt = Batch(tb, cuda, [80, 1400], [n, n], page=16, heads=1, dim=64, typ="bf16", seed=34)
     bt.fill_fast()
     q, _ = bt.queries(2)
-    clean = bt.attend(q, 2, 0.1)[0].clone()
+    clean = bt.attend(q, 2, 0.1, max_len=max_len)[0].clone()
     q[n, 3] = float("nan")
-    out, lse = bt.attend(q, 2, 0.1)
+    out, lse = bt.attend(q, 2, 0.1, max_len=max_len)
     assert bool(out[n, :64].isnan().all()) and bool(lse[n, 0].isnan())
     same = cuda.ones_like(out, dtype=cuda.bool)
     same[n, :64] = False
     assert cuda.equal(out[same], clean[same])
 
 
+@pytest.mark.parametrize("max_len", [None, LONG])
 @pytest.mark.parametrize("n", [2, 40])
-def test_rows_that_see_nothing(tb, cuda, n):
+def test_rows_that_see_nothing(tb, cuda, max_len, n):
     """More rows than tokens: the rows before the first token are zero, lse -inf.
     Sequences without tokens."""
     bt = Batch(tb, cuda, [5, 0, 3], [5, 0, 3], page=16, heads=1, dim=64, seed=35)
@@ -528,14 +536,15 @@ def test_rows_that_see_nothing(tb, cuda, n):
     bt.total = 2 * n + 1
     bt.index()
     q, _ = bt.queries(2)
-    out, lse = bt.attend(q, 2, 0.1)
+    out, lse = bt.attend(q, 2, 0.1, max_len=max_len)
     bt.check(out, lse, q, 2, 0.1)
     assert bool((out[:n - 1] == 0).all()) and bool(cuda.isneginf(lse[:n - 1]).all())
     assert bool((out[n:2 * n] == 0).all()) and bool((out[2 * n:] == 7).all())
 
 
+@pytest.mark.parametrize("max_len", [None, LONG])
 @pytest.mark.parametrize("n", [1, 3, 40])
-def test_pages_outside_the_cache_are_not_seen(tb, cuda, n):
+def test_pages_outside_the_cache_are_not_seen(tb, cuda, max_len, n):
     lens = [100, 1500]
     bt = Batch(tb, cuda, lens, [n, n], page=16, heads=1, dim=64, seed=36)
     bt.fill_fast()
@@ -543,7 +552,7 @@ def test_pages_outside_the_cache_are_not_seen(tb, cuda, n):
     good = bt.table.copy()
     bt.table[0, 2], bt.table[1, 5], bt.table[1, 60] = bt.host.pages, -1, 2 ** 31 - 1
     bt.index()
-    out, lse = bt.attend(q, 2, 0.1)
+    out, lse = bt.attend(q, 2, 0.1, max_len=max_len)
     assert tb.device_error() == 2
     for b, hidden in ((0, [2]), (1, [5, 60])):
         keep = [p for p in range(lens[b]) if p // 16 not in hidden]
@@ -567,7 +576,7 @@ def test_lengths_outside_the_table(tb, cuda):
     q, _ = bt.queries(2)
     out0 = bt.attend(q, 2, 0.1)[0].clone()
     for bad in (10 ** 9, -4, 2 ** 31 - 1, -2 ** 31):
-        for max_len in (100, 5000):
+        for max_len in (100, LONG):
             bt.d_lens[1] = bad
             out, _ = bt.attend(q, 2, 0.1, max_len=max_len)
             assert tb.device_error() == 2
@@ -579,7 +588,7 @@ def test_more_rows_than_max_rows_is_reported(tb, cuda):
     bt = Batch(tb, cuda, [2000, 90], [40, 40], page=16, heads=1, dim=64, seed=38)
     bt.fill_fast()
     q, _ = bt.queries(2)
-    for max_len in (100, 2000):
+    for max_len in (100, LONG):
         bt.attend(q, 2, 0.1, max_rows=1, max_len=max_len)
         assert tb.device_error() == 4
 
@@ -592,34 +601,36 @@ def test_bounds_may_be_loose(tb, cuda, max_rows, max_len):
     bt.run(4, max_rows=max_rows, max_len=max_len)
 
 
+@pytest.mark.parametrize("max_len", [None, LONG])
 @pytest.mark.parametrize("n", [1, 6, 40])
-def test_strides_and_no_lse(tb, cuda, n):
+def test_strides_and_no_lse(tb, cuda, max_len, n):
     bt = Batch(tb, cuda, [60, 1300], [n, n], page=32, heads=2, dim=64, stride=2 * 32 * 72 + 4096, seed=40, pad=1)
     bt.fill_fast()
     wide, q = bt.queries(4, stride=4 * 64 + 24)
-    out, _ = bt.attend(wide, 4, 0.125, lse=False, q_stride=4 * 64 + 24, out_stride=4 * 64 + 40)
+    out, _ = bt.attend(wide, 4, 0.125, lse=False, q_stride=4 * 64 + 24, out_stride=4 * 64 + 40, max_len=max_len)
     bt.check(out, None, q, 4, 0.125)
     assert bool((out[:, 256:] == 7).all())
 
 
+@pytest.mark.parametrize("max_len", [2100, LONG])
 @pytest.mark.parametrize("n", [1, 6, 40])
-def test_same_bits_again_and_in_a_graph(tb, cuda, n):
+def test_same_bits_again_and_in_a_graph(tb, cuda, n, max_len):
     """Two runs, a captured one and its replays give the same bits; a replay
     follows the lengths, rows and table that the device holds then."""
     bt = Batch(tb, cuda, [900, 2100, 30], [n, n, n], page=16, heads=2, dim=128, seed=41)
     bt.fill_fast()
     q, _ = bt.queries(8)
-    out0, lse0 = (x.clone() for x in bt.attend(q, 8, 0.09))
-    out1, lse1 = bt.attend(q, 8, 0.09)
+    out0, lse0 = (x.clone() for x in bt.attend(q, 8, 0.09, max_len=max_len))
+    out1, lse1 = bt.attend(q, 8, 0.09, max_len=max_len)
     assert cuda.equal(out0, out1) and cuda.equal(lse0, lse1)
-    need = tb.kv4_attention_workspace(bt.cache, bt.rows, 8, n, 2100)
+    need = tb.kv4_attention_workspace(bt.cache, bt.rows, 8, n, max_len)
     ws = cuda.empty(max(need, 16), dtype=cuda.uint8, device="cuda")
     out, lse = cuda.zeros_like(out0), cuda.zeros_like(lse0)
     s = cuda.cuda.Stream()
     graph = cuda.cuda.CUDAGraph()
     s.wait_stream(cuda.cuda.current_stream())
     with cuda.cuda.graph(graph, stream=s):
-        tb.kv4_attention(bt.cache, bt.rows, tb.Format.F16, q, out, lse, 8, n, 2100, 0.09, workspace=ws,
+        tb.kv4_attention(bt.cache, bt.rows, tb.Format.F16, q, out, lse, 8, n, max_len, 0.09, workspace=ws,
                          workspace_bytes=need)
     graph.replay()
     cuda.cuda.synchronize()
@@ -631,7 +642,7 @@ def test_same_bits_again_and_in_a_graph(tb, cuda, n):
     cuda.cuda.synchronize()
     bt.check(out, lse, q, 8, 0.09)
     # the eager call follows too
-    out1, lse1 = bt.attend(q, 8, 0.09, max_len=2100)
+    out1, lse1 = bt.attend(q, 8, 0.09, max_len=max_len)
     assert cuda.equal(out, out1) and cuda.equal(lse, lse1)
 
 
@@ -641,14 +652,14 @@ def test_streams_side_by_side(tb, cuda):
     for bt in bts:
         bt.fill_fast()
     qs = [bt.queries(8)[0] for bt in bts]
-    need = tb.kv4_attention_workspace(bts[0].cache, bts[0].rows, 8, 1, 3000)
+    need = tb.kv4_attention_workspace(bts[0].cache, bts[0].rows, 8, 1, LONG)
     outs = [cuda.zeros((2, 1024), dtype=cuda.float16, device="cuda") for _ in bts]
     wss = [cuda.empty(need, dtype=cuda.uint8, device="cuda") for _ in bts]
     cuda.cuda.synchronize()
     streams = [cuda.cuda.Stream() for _ in bts]
     for _ in range(20):
         for bt, q, out, ws, st in zip(bts, qs, outs, wss, streams):
-            tb.kv4_attention(bt.cache, bt.rows, tb.Format.F16, q, out, None, 8, 1, 3000, 0.09, workspace=ws,
+            tb.kv4_attention(bt.cache, bt.rows, tb.Format.F16, q, out, None, 8, 1, LONG, 0.09, workspace=ws,
                              workspace_bytes=need, stream=st)
     cuda.cuda.synchronize()
     for bt, q, out in zip(bts, qs, outs):
@@ -658,13 +669,13 @@ def test_streams_side_by_side(tb, cuda):
 def test_workspace_is_asked_for(tb, cuda):
     bt = Batch(tb, cuda, [3000], [1], page=16, heads=1, dim=64, seed=60)
     q, _ = bt.queries(2)
-    need = tb.kv4_attention_workspace(bt.cache, bt.rows, 2, 1, 3000)
+    need = tb.kv4_attention_workspace(bt.cache, bt.rows, 2, 1, LONG)
     assert need > 0
     out = cuda.zeros((1, 128), dtype=cuda.float16, device="cuda")
     ws = cuda.empty(need + 16, dtype=cuda.uint8, device="cuda")
     for w, nb, st in ((None, 0, "WORKSPACE"), (ws, need - 1, "WORKSPACE"), (ws.data_ptr() + 4, need, "ALIGNMENT")):
         with pytest.raises(tb.TBError) as e:
-            tb.kv4_attention(bt.cache, bt.rows, tb.Format.F16, q, out, None, 2, 1, 3000, 0.1, workspace=w, workspace_bytes=nb)
+            tb.kv4_attention(bt.cache, bt.rows, tb.Format.F16, q, out, None, 2, 1, LONG, 0.1, workspace=w, workspace_bytes=nb)
         assert e.value.status == tb.Status[st]
 
 
