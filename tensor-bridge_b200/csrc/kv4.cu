@@ -247,7 +247,7 @@ template <int D, bool BF16>
 cudaError_t run_prompt(const Kv4Attn& a, cudaStream_t st) {
     using C = PromptCfg<D>;
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = prepare_kernel(k_kv4_prompt<C, BF16>, C::SMEM, 0, done);
+    cudaError_t e = prepare_kernel(k_kv4_prompt<C, BF16>, C::SMEM, C::REGS, done);
     if (e != cudaSuccess) return e;
     const unsigned units = static_cast<unsigned>(a.rows.batch) * a.cache.heads * a.prompt_tiles;
     e = launch_early(k_kv4_prompt<C, BF16>, dim3(units * a.prompt_splits), kPromptThreads, C::SMEM, st, a);

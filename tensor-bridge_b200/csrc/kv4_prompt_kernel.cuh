@@ -8,9 +8,10 @@
 //                     to the same TMEM columns
 //   O_t += P_t V      tcgen05.mma, P_t from TMEM, V from shared memory
 // While one tile's rows take their exponentials the tensor core works for the
-// other.  K and V arrive as codes (bulk copies, one per page where a page is
-// at most a tile) and four warps turn them into FP16 operand tiles once per
-// 256 rows; a thread owns one token of the tile.
+// other: P_0 V, the next S_0, P_1 V, the next S_1.  K and V arrive as codes
+// (bulk copies, one per page where a page is at most a tile) and eight warps,
+// four for each, turn them into FP16 operand tiles once per 256 rows; a thread
+// owns one token of the tile.
 //
 // Layout: K, V and Q tiles are [row][64 d] panels of 128-byte rows under the
 // 128-byte swizzle.  The same picture is K-major for Q K^T and, as [token][d],
@@ -18,11 +19,11 @@
 // the converter second value first; Q is stored in the same order, and the
 // output's columns are swapped back when they are read.
 //
-// The maximum m of a row is moved only when a score passes it by 2^8, so the
-// usual tile takes one pass: exponentials with the old m, the largest score
-// found along the way, and a second pass (with O scaled in TMEM) only if it
-// passed.  S_t of the next tile is issued behind P_t V of this one, so a row's
-// thread that sees S_t finds O_t at rest.
+// The maximum m of a row is moved only when a score passes it by 2^8 (2^15 in
+// the second half of a tile), so the usual tile takes one pass: exponentials
+// with the old m, the largest score found along the way, and a second pass
+// (with O scaled in TMEM) only if it passed.  S_t of a tile is issued behind
+// P_t V of the tile before, so a thread that sees S_t finds O_t at rest.
 //
 // TMEM (512 columns): S_0, S_1 (128 each, P in the first 64), O_0, O_1 (D each).
 #pragma once
@@ -33,7 +34,7 @@ namespace tb {
 
 constexpr int kPromptRows = 256;
 constexpr int kPromptTile = 128;                    // tokens
-constexpr int kPromptThreads = 512;                 // 8 softmax, 4 decode, MMA, loader, 2 idle warps
+constexpr int kPromptThreads = 640;                 // warps: 8 softmax, 4 decode K, 4 decode V, MMA, loader, 2 idle
 
 template <int D_>
 struct PromptCfg {
@@ -48,24 +49,23 @@ struct PromptCfg {
     static constexpr int OFF_SLOT = 2 * OPERAND;
     static constexpr int OFF_RAW = OFF_SLOT + SLOTS * OPERAND;
     static constexpr int OFF_BAR = OFF_RAW + NR * RAW;
-    static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment of the base
+    static constexpr int OFF_QSCALE = OFF_BAR + 256;
+    static constexpr int SMEM = OFF_QSCALE + kPromptRows * 4 + 1024;  // + alignment of the base
     static constexpr int S_COLS = 128;
     static constexpr int O_COL = 256;
+    // Registers a thread: at launch, then by role.
+    static constexpr int REGS = 96, REGS_SOFTMAX = 152, REGS_DECODE = 64, REGS_REST = 40;
+    static_assert(256 * (REGS_SOFTMAX + REGS_DECODE) + 128 * REGS_REST <= kPromptThreads * REGS, "registers of the launch");
     static constexpr int SLOT_FLOATS = kPromptRows * (D + 2);
 };
 
-// Descriptor of an N-major operand tile (V as [token][d]): 64 values of N are
-// a 128-byte row, 8 rows of K an atom of 1024 bytes (the stride byte offset),
-// 64 more values of N a panel (the leading byte offset).
+// Low word of the descriptor of an N-major operand tile (V as [token][d]): 64
+// values of N are a 128-byte row, 8 rows of K an atom of 1024 bytes (the stride
+// byte offset, in the high word), 64 more values of N a panel (the leading byte
+// offset).
 template <class C>
-__device__ __forceinline__ uint64_t sdesc_v(uint32_t addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>((C::PANEL >> 4) & 0x3FFFu) << 16;
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;
-    d |= static_cast<uint64_t>(1u) << 46;
-    d |= static_cast<uint64_t>(2u) << 61;
-    return d;
+__device__ __forceinline__ uint32_t sdesc_v_lo(uint32_t addr) {
+    return ((addr >> 4) & 0x3FFFu) | (static_cast<uint32_t>(C::PANEL >> 4) << 16);
 }
 
 // Whether the prompt kernel takes a sequence: more packed rows than the step
@@ -102,24 +102,30 @@ __device__ __forceinline__ PromptUnit prompt_unit(const Kv4Attn& a, int unit, in
     u.last_pos = u.q.pos0 + (u.row_base + u.row_count - 1) / a.group;
     u.span = kv4_span(u.first_pos, u.last_pos, u.q.len, a.window, a.sinks, 7);
     const int tiles = kv4_span_chunks(u.span);
-    u.t0 = static_cast<int>(static_cast<long long>(tiles) * split / a.prompt_splits);
-    u.t1 = static_cast<int>(static_cast<long long>(tiles) * (split + 1) / a.prompt_splits);
+    u.t0 = 0;
+    u.t1 = tiles;
+    if (a.prompt_splits > 1) {
+        u.t0 = static_cast<int>(static_cast<long long>(tiles) * split / a.prompt_splits);
+        u.t1 = static_cast<int>(static_cast<long long>(tiles) * (split + 1) / a.prompt_splits);
+    }
     return u;
 }
 
-// Bit g set where granule g (16 tokens, or a page's share of the tile if that
-// is more) of the tile at token `tok0` has a page of the cache; bits of tokens
-// behind the sequence stay clear.  The whole warp calls it; lane g looks at
-// granule g.  *page is the lane's page number.
-__device__ __forceinline__ uint32_t prompt_pages(const Kv4Attn& a, const PromptUnit& u, int tok0, int* page) {
+// A tile's pages.  Granule g is 16 tokens, or a page's share of the tile if
+// that is more; lane g looks it up.  prompt_look only loads the lane's page
+// number (-2 behind the sequence), so that a tile's can be on its way while the
+// tile before is worked on; prompt_pages then gives the word in which bit g is
+// set where granule g has a page of the cache.  The whole warp calls them.
+__device__ __forceinline__ int prompt_look(const Kv4Attn& a, const PromptUnit& u, int j) {
+    if (j >= u.t1) return -2;
     const int lane = threadIdx.x & 31;
     const int shift = a.cache.page_shift, gshift = shift < 7 ? shift : 7;
-    const int tok = tok0 + (lane << gshift);
-    int p = -1;
-    const bool inside = (lane << gshift) < kPromptTile && tok < u.q.len;
-    if (inside) p = a.rows.table[static_cast<size_t>(u.b) * a.rows.width + (tok >> shift)];
-    *page = p;
-    return __ballot_sync(0xFFFFFFFFu, inside && kv4_page_ok(a.cache, p));
+    const int tok = kv4_span_chunk(u.span, j) * kPromptTile + (lane << gshift);
+    if ((lane << gshift) >= kPromptTile || tok >= u.q.len) return -2;
+    return a.rows.table[static_cast<size_t>(u.b) * a.rows.width + (tok >> shift)];
+}
+__device__ __forceinline__ uint32_t prompt_pages(const Kv4Attn& a, int page) {
+    return __ballot_sync(0xFFFFFFFFu, kv4_page_ok(a.cache, page));
 }
 
 // Whether every row of the unit sees the whole tile and all of it has pages.
@@ -138,45 +144,62 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
     return (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
 }
 
-// One pass over the thread's 128 scores: p = 2^(s f - m), hidden ones 0.
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void fma_f32x2(float& x0, float& x1, float s0, float s1, uint64_t f, uint64_t c) {
+    asm("{\n\t.reg .b64 s, r;\n\tmov.b64 s, {%2, %3};\n\tfma.rn.f32x2 r, s, %4, %5;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(x0), "=f"(x1) : "f"(s0), "f"(s1), "l"(f), "l"(c));
+}
+__device__ __forceinline__ void add_f32x2(float& a0, float& a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
+
+// One pass over the thread's 64 scores: p = 2^(s f - m), hidden ones 0.
 // Returns the largest s f - m; *sum gets the sum of p.
 template <bool MASKED>
-__device__ __forceinline__ float prompt_pass(uint32_t s_tmem, float f, float m, const uint32_t (&mask)[4],
-                                             uint32_t (&p)[64], float* sum) {
+__device__ __forceinline__ float prompt_pass(uint32_t s_tmem, float f, float m, uint32_t mask0, uint32_t mask1,
+                                             uint32_t (&p)[32], float* sum) {
+    uint32_t s[2][32];
+    tmem_ld_32x32b_x32(s_tmem, s[0]);
+    tmem_ld_32x32b_x32(s_tmem + 32, s[1]);
+    tmem_wait_ld();
     float top = -INFINITY, t0 = 0.0f, t1 = 0.0f;
+    const uint64_t ff = pack_f32x2(f, f), mm = pack_f32x2(-m, -m);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t s[32];
-        tmem_ld_32x32b_x32(s_tmem + 32 * c, s);
-        tmem_wait_ld();
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-            float x0 = fmaf(__uint_as_float(s[i]), f, -m), x1 = fmaf(__uint_as_float(s[i + 1]), f, -m);
+            float x0, x1;
+            fma_f32x2(x0, x1, __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]), ff, mm);
             if constexpr (MASKED) {
-                x0 = (mask[c] >> i) & 1u ? x0 : -INFINITY;
-                x1 = (mask[c] >> (i + 1)) & 1u ? x1 : -INFINITY;
+                x0 = ((c ? mask1 : mask0) >> i) & 1u ? x0 : -INFINITY;
+                x1 = ((c ? mask1 : mask0) >> (i + 1)) & 1u ? x1 : -INFINITY;
             }
             top = fmaxf(top, fmaxf(x0, x1));
             x0 = ex2(x0);
             x1 = ex2(x1);
-            t0 += x0;
-            t1 += x1;
+            add_f32x2(t0, t1, x0, x1);
             p[16 * c + i / 2] = pack_half2(x0, x1);
         }
-    }
     *sum = t0 + t1;
     return top;
 }
 
 // The largest s f of the thread's row that is not hidden.
-__device__ __noinline__ float prompt_top(uint32_t s_tmem, float f, const uint32_t (&mask)[4], bool open) {
+__device__ __noinline__ float prompt_top(uint32_t s_tmem, float f, uint32_t mask0, uint32_t mask1) {
     float top = -INFINITY;
 #pragma unroll 1
-    for (int c = 0; c < 8; ++c) {
+    for (int c = 0; c < 4; ++c) {
         uint32_t s[16];
         tmem_ld_32x32b_x16(s_tmem + 16 * c, s);
         tmem_wait_ld();
-        const uint32_t w = open ? 0xFFFFu : mask[c / 2] >> (16 * (c & 1));
+        const uint32_t w = (c < 2 ? mask0 : mask1) >> (16 * (c & 1));
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, (w >> i) & 1u ? __uint_as_float(s[i]) * f : -INFINITY);
     }
@@ -200,8 +223,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
     uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_ptr + 1);
     volatile int* nan_seen = abort + 1;
+    float* q_scale = reinterpret_cast<float*>(smem + C::OFF_QSCALE);  // score -> log2 units, per row
 
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    // A value that a shuffle or a vote gives is the same in the whole warp for
+    // the compiler too, which then keeps what follows from it in uniform
+    // registers: MMAs are issued from those.
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid / 32, 0), lane = tid & 31;
     const int unit = blockIdx.x / a.prompt_splits, split = blockIdx.x - unit * a.prompt_splits;
     const PromptUnit u = prompt_unit(a, unit, split);
     const int tiles = u.any ? u.t1 - u.t0 : 0;
@@ -214,7 +241,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
     if (tid == 0) {
         for (int i = 0; i < C::NR; ++i) {
             mbar_init(&raw_full[i], 1);
-            mbar_init(&raw_empty[i], 4);
+            mbar_init(&raw_empty[i], 8);
         }
         for (int i = 0; i < C::SLOTS; ++i) {
             mbar_init(&op_full[i], 4);
@@ -234,7 +261,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         if (static_cast<long long>(u.q.n) * a.group > static_cast<long long>(a.prompt_tiles) * kPromptRows)
             atomicOr(&g_tb_device_error, kErrRows);
     }
-    if (warp == 12) tmem_alloc(tmem_ptr, 512);
+    if (warp == 16) tmem_alloc(tmem_ptr, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -246,6 +273,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
     const uint32_t gbytes = gtok * C::TOKEN_BYTES * 2;
 
     if (warp < 8) {
+        reg_inc<C::REGS_SOFTMAX>();
         // ---- softmax: thread = row ----------------------------------------------------
         const int t = warp / 4, r = tid & 127;
         if (t < act) {
@@ -254,63 +282,68 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             const int i = row / a.group;
             const int pos = u.q.pos0 + i;
             const int h = u.head * a.group + row - i * a.group;
-            // Q into its tile, pairs swapped; BF16 scaled as in the step kernel.
-            float f = fmaxf(fabsf(a.scale_log2), 1e-37f);  // positive, its sign in q, as in the step kernel
-            const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+            // Q into its tile, pairs swapped; BF16 scaled and the sign of the
+            // factor moved as in the step kernel.  D / 8 lanes load a row.
             {
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                                  (u.q.first + i) * a.q_stride +
-                                                                  static_cast<long long>(h) * D);
-                float up = 1.0f, up2 = 1.0f;
-                if constexpr (BF16) {
-                    uint32_t e = 0;
-                    if (valid) {
+                constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
+                const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+                const int k = lane % LANES;  // 16-byte chunk of the row
+                uint4 v[32 / AT_ONCE];
 #pragma unroll
-                        for (int k = 0; k < D / 8; ++k) {
-                            const uint4 v = src[k];
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) e = max(e, max((w[j] >> 7) & 0xFFu, (w[j] >> 23) & 0xFFu));
-                        }
+                for (int x = 0; x < 32 / AT_ONCE; ++x) {
+                    const int rr = (warp & 3) * 32 + x * AT_ONCE + lane / LANES;
+                    v[x] = make_uint4(0u, 0u, 0u, 0u);
+                    if (t * 128 + rr < u.row_count) {
+                        const int ro = u.row_base + t * 128 + rr, to = ro / a.group;
+                        v[x] = *reinterpret_cast<const uint4*>(
+                            static_cast<const uint16_t*>(a.q) + (u.q.first + to) * a.q_stride +
+                            static_cast<long long>(u.head * a.group + ro - to * a.group) * D + 8 * k);
                     }
-                    const int k = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = k > 120 ? 120 : k, k2 = k - k1;
-                    up = exp2i(k1);
-                    up2 = exp2i(k2);
-                    f = fmaxf((f * exp2i(-k1)) * exp2i(-k2), 1e-37f);
                 }
                 uint8_t* q_tile = smem + t * C::OPERAND;
 #pragma unroll
-                for (int k = 0; k < D / 8; ++k) {
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (valid) v = src[k];
-                    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                for (int x = 0; x < 32 / AT_ONCE; ++x) {
+                    const int rr = (warp & 3) * 32 + x * AT_ONCE + lane / LANES;
+                    uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+                    float f = fmaxf(fabsf(a.scale_log2), 1e-37f);
+                    if constexpr (BF16) {
+                        uint32_t e = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if constexpr (BF16)
+                        for (int j = 0; j < 4; ++j) e = max(e, max((w[j] >> 7) & 0xFFu, (w[j] >> 23) & 0xFFu));
+#pragma unroll
+                        for (int d = 1; d < LANES; d <<= 1) e = max(e, __shfl_xor_sync(0xFFFFFFFFu, e, d));
+                        const int kk = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = kk > 120 ? 120 : kk, k2 = kk - k1;
+                        const float up = exp2i(k1), up2 = exp2i(k2);
+                        f = fmaxf((f * exp2i(-k1)) * exp2i(-k2), 1e-37f);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
                             w[j] = pack_half2(__uint_as_float(w[j] & 0xFFFF0000u) * up * up2,
                                               __uint_as_float(w[j] << 16) * up * up2);
-                        else
-                            w[j] = prmt(w[j], 0u, 0x1032u);
-                        w[j] ^= sign;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[j] = prmt(w[j], 0u, 0x1032u);
                     }
-                    *reinterpret_cast<uint4*>(q_tile + (k / 8) * C::PANEL + r * 128 + (((k & 7) ^ (r & 7)) << 4)) =
-                        make_uint4(w[0], w[1], w[2], w[3]);
+                    if (k == 0) q_scale[t * 128 + rr] = f;
+                    *reinterpret_cast<uint4*>(q_tile + (k / 8) * C::PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) =
+                        make_uint4(w[0] ^ sign, w[1] ^ sign, w[2] ^ sign, w[3] ^ sign);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[t]);
             }
+            const float f = q_scale[t * 128 + r];  // written by this warp
 
             const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane offset 32 * (warp % 4)
             const uint32_t s_tmem = tmem + quarter + t * C::S_COLS;
             const uint32_t o_tmem = tmem + quarter + C::O_COL + t * D;
             float m = kNoMax, l = 0.0f;
             bool ok = true;
+            int page = prompt_look(a, u, u.t0);
             for (int j = 0; j < tiles && ok; ++j) {
                 const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
-                int page;
-                const uint32_t pages = prompt_pages(a, u, tok0, &page);
+                const uint32_t pages = prompt_pages(a, page);
                 const bool open = prompt_open(a, u, tok0, pages);
+                page = prompt_look(a, u, u.t0 + j + 1);
                 uint32_t mask[4];
                 if (!open) {
 #pragma unroll
@@ -328,43 +361,57 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                         mask[c] = w & there;
                     }
                 }
-                ok = mbar_wait(&s_full[t], j & 1, abort);
-                if (!__all_sync(0xFFFFFFFFu, ok)) break;
-                tc_fence_after();
-                uint32_t p[64];
-                float sum;
-                const float top = open ? prompt_pass<false>(s_tmem, f, m, mask, p, &sum)
-                                       : prompt_pass<true>(s_tmem, f, m, mask, p, &sum);
-                const bool move = top > 8.0f;
-                if (__any_sync(0xFFFFFFFFu, move)) {
-                    // The new m is the row's largest score, found anew: s f - m
-                    // has lost it where m was kNoMax.
-                    const float y = prompt_top(s_tmem, f, mask, open);
-                    const float m_new = move ? y : m;
-                    const float scale = ex2(m - m_new);
-                    m = m_new;
-                    l *= scale;
-                    if (open) prompt_pass<false>(s_tmem, f, m, mask, p, &sum);
-                    else prompt_pass<true>(s_tmem, f, m, mask, p, &sum);
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {
-                            uint32_t o[16];
-                            tmem_ld_32x32b_x16(o_tmem + c, o);
-                            tmem_wait_ld();
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[t], j & 1, abort));
+                if (!ok) break;
+                tc_fence_after();  // S_t is there, and O_t at rest: its last P V came before
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * scale);
-                            tmem_st_32x32b_x16(o_tmem + c, o);
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t s_half = s_tmem + 64 * half;
+                    const uint32_t m0 = open ? 0xFFFFFFFFu : mask[2 * half], m1 = open ? 0xFFFFFFFFu : mask[2 * half + 1];
+                    uint32_t p[32];
+                    float sum;
+                    float top = open ? prompt_pass<false>(s_half, f, m, m0, m1, p, &sum)
+                                     : prompt_pass<true>(s_half, f, m, m0, m1, p, &sum);
+                    // The first half keeps P below 2^8, the second below 2^15:
+                    // moving m there also means P of the first half again.
+                    if (__any_sync(0xFFFFFFFFu, top > (half == 0 ? 8.0f : 15.0f))) {
+                        // The row's largest score, found anew: s f - m has lost
+                        // it where m was kNoMax.  m stays a whole number, so
+                        // that what is scaled by its steps is not rounded.
+                        const float m_new = fmaxf(m, ceilf(prompt_top(s_half, f, m0, m1)));
+                        const float step = m_new - m;
+                        const float scale = step < 126.0f ? exp2i(-static_cast<int>(step)) : 0.0f;
+                        m = m_new;
+                        l *= scale;
+                        if (open) prompt_pass<false>(s_half, f, m, m0, m1, p, &sum);
+                        else prompt_pass<true>(s_half, f, m, m0, m1, p, &sum);
+                        if (half == 1) {
+                            const uint32_t by = pack_half2(scale, scale);
+                            tmem_wait_st();
+#pragma unroll 1
+                            for (int c = 0; c < 32; c += 16) {
+                                uint32_t o[16];
+                                tmem_ld_32x32b_x16(s_tmem + c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = hmul2(o[k], by);
+                                tmem_st_32x32b_x16(s_tmem + c, o);
+                            }
+                        }
+                        if (j > 0) {
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t o[16];
+                                tmem_ld_32x32b_x16(o_tmem + c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * scale);
+                                tmem_st_32x32b_x16(o_tmem + c, o);
+                            }
                         }
                     }
-                }
-                l += sum;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) w[k] = p[16 * c + k];
-                    tmem_st_32x32b_x16(s_tmem + 16 * c, w);
+                    l += sum;
+                    tmem_st_32x32b_x32(s_tmem + 32 * half, p);  // over scores that have been read
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -374,7 +421,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
 
             // ---- the rows' result --------------------------------------------------------
             ok = mbar_wait(&o_full[t], 0, abort);
-            named_bar_sync(1, 128 + 128 * act);  // the decode warps have recorded their NaN blocks
+            named_bar_sync(1, 256 + 128 * act);  // the decode warps have recorded their NaN blocks
             if (__all_sync(0xFFFFFFFFu, ok)) {
                 tc_fence_after();
                 uint32_t nan_blocks = 0;
@@ -444,28 +491,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                 }
             }
         }
-    } else if (warp < 12) {
-        // ---- decode: thread = token of the tile ------------------------------------------
+    } else if (warp < 16) {
+        reg_dec<C::REGS_DECODE>();
+        // ---- decode: thread = token of the tile; four warps for K, four for V -------------
+        const int kv = (warp - 8) / 4;
         const uint32_t tok = static_cast<uint32_t>(tid & 127);
         const uint32_t g0 = (tok >> gshift) * gbytes, place = tok & (gtok - 1u);
-        uint32_t n_op = 0;
         bool ok = true;
+        int page = prompt_look(a, u, u.t0);
         for (int j = 0; j < tiles && ok; ++j) {
             const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
-            int page;
-            const uint32_t pages = prompt_pages(a, u, tok0, &page);
+            const uint32_t pages = prompt_pages(a, page);
             const bool open = prompt_open(a, u, tok0, pages);
+            page = prompt_look(a, u, u.t0 + j + 1);
             const bool there = ((pages >> (tok >> gshift)) & 1u) && tok0 + static_cast<int>(tok) < u.q.len;
             const int st = j % C::NR;
             ok = mbar_wait(&raw_full[st], (j / C::NR) & 1, abort);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            const uint32_t n_op = 2 * j + kv;  // K_0, V_0, K_1, ... take the slots in turn
+            const int slot = n_op % C::SLOTS;
+            ok = ok && (n_op < C::SLOTS || mbar_wait(&op_empty[slot], (n_op / C::SLOTS - 1) & 1, abort));
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
             const uint8_t* raw = smem + C::OFF_RAW + st * C::RAW + g0;
-#pragma unroll 1
-            for (int kv = 0; kv < 2; ++kv, ++n_op) {
-                const int slot = n_op % C::SLOTS;
-                ok = n_op < C::SLOTS || mbar_wait(&op_empty[slot], (n_op / C::SLOTS - 1) & 1, abort);
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                if (!ok) break;
+            {
                 uint8_t* dst = smem + C::OFF_SLOT + slot * C::OPERAND + tok * 128;
                 const uint8_t* codes = raw + (kv ? at_vc : 0u) + place * (D / 2);
                 const uint8_t* scales = raw + (kv ? at_vs : at_ks) + place * (D / 16);
@@ -516,83 +564,103 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&op_full[slot]);
-                    if (kv) mbar_arrive(&raw_empty[st]);
+                    mbar_arrive(&raw_empty[st]);
                 }
             }
         }
-        named_bar_sync(1, 128 + 128 * act);
-    } else if (warp == 12) {
-        // ---- tensor core ------------------------------------------------------------------
+        named_bar_sync(1, 256 + 128 * act);
+    } else {
+      reg_dec<C::REGS_REST>();
+      if (warp == 16) {
+        // ---- tensor core: the warp waits, one lane issues ---------------------------------
+        // All 512 columns are this CTA's, so its tensor memory starts at column 0.
         constexpr uint32_t idesc_s = idesc_make(0, 0, 128, 128);
         constexpr uint32_t idesc_o = idesc_make(0, 0, 128, D) | (1u << 16);  // V is N-major
-        const uint32_t q0 = smem_addr(smem), slot0 = smem_addr(smem + C::OFF_SLOT);
-        bool ok = true;
+        const uint32_t q_lo = sdesc_lo(smem_addr(smem));
+        const uint32_t k_lo = sdesc_lo(smem_addr(smem + C::OFF_SLOT)), v_lo = sdesc_v_lo<C>(smem_addr(smem + C::OFF_SLOT));
+        const int n = __reduce_max_sync(0xFFFFFFFFu, tiles);
+        const bool two = __any_sync(0xFFFFFFFFu, act == 2);
+        bool ok = __all_sync(0xFFFFFFFFu, tmem == 0u);
+        if (!ok && lane == 0) {
+            atomicOr(&g_tb_device_error, kErrTimeout);
+            *abort = 1;
+        }
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = ok && mbar_wait(bar, parity, abort);
-            ok = __all_sync(0xFFFFFFFFu, ok);
+            ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(bar, parity, abort));
             tc_fence_after();
             return ok;
         };
-        auto scores = [&](int t, uint32_t op) {
-            if (elect_one()) {
-                const uint32_t kb = slot0 + (op % C::SLOTS) * C::OPERAND, qb = q0 + t * C::OPERAND;
+        // S_t = Q_t K^T with the K tile in `slot`.
+        auto scores = [&](int t, uint32_t slot) {
+            const uint32_t ql = q_lo + t * (C::OPERAND >> 4), kl = k_lo + slot * (C::OPERAND >> 4);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t at = (k / 4) * C::PANEL + (k % 4) * 32;
-                    mma_f16_ss(tmem + t * C::S_COLS, sdesc_make(sdesc_lo(qb + at)), sdesc_make(sdesc_lo(kb + at)), idesc_s,
-                               k > 0);
-                }
-                mma_commit(&s_full[t]);
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t at = ((k / 4) * C::PANEL + (k % 4) * 32) >> 4;
+                mma_f16_ss(t * C::S_COLS, sdesc_make(ql + at), sdesc_make(kl + at), idesc_s, k > 0);
             }
-            __syncwarp();
+            mma_commit(&s_full[t]);
         };
-        auto values = [&](int t, uint32_t op, bool first) {
-            if (elect_one()) {
-                const uint32_t vb = slot0 + (op % C::SLOTS) * C::OPERAND;
+        auto values = [&](int t, uint32_t slot, uint32_t accumulate) {
+            const uint32_t vl = v_lo + slot * (C::OPERAND >> 4);
 #pragma unroll
-                for (int k = 0; k < kPromptTile / 16; ++k)
-                    mma_f16_ts(tmem + C::O_COL + t * D, tmem + t * C::S_COLS + 8 * k, sdesc_v<C>(vb + k * 2048), idesc_o,
-                               !(first && k == 0));
+            for (int k = 0; k < kPromptTile / 16; ++k)
+                mma_f16_ts(C::O_COL + t * D, t * C::S_COLS + 8 * k, sdesc_make(vl + k * (2048 >> 4)), idesc_o,
+                           k > 0 ? 1u : accumulate);
+        };
+        wait(&q_full[0], 0);
+        if (two) wait(&q_full[1], 0);
+        if (wait(&op_full[0], 0)) {
+            if (elect_one()) {
+                scores(0, 0);
+                if (two) scores(1, 0);
+                mma_commit(&op_empty[0]);
             }
             __syncwarp();
-        };
-        auto release = [&](uint64_t* bar) {
-            if (elect_one()) mma_commit(bar);
-            __syncwarp();
-        };
-        for (int t = 0; t < act && ok; ++t) wait(&q_full[t], 0);
-        if (ok && wait(&op_full[0], 0)) {
-            for (int t = 0; t < act; ++t) scores(t, 0);
-            release(&op_empty[0]);
         }
-        for (int j = 0; j < tiles && ok; ++j) {
-            const uint32_t v_op = 2 * j + 1, k_op = 2 * j + 2;
-            for (int t = 0; t < act && ok; ++t) {
-                if (t == 0 && !wait(&op_full[v_op % C::SLOTS], (v_op / C::SLOTS) & 1)) break;
-                if (!wait(&p_full[t], j & 1)) break;
-                values(t, v_op, j == 0);
-                if (t == act - 1) release(&op_empty[v_op % C::SLOTS]);
-                if (j + 1 < tiles) {
-                    if (t == 0 && !wait(&op_full[k_op % C::SLOTS], (k_op / C::SLOTS) & 1)) break;
-                    scores(t, k_op);
-                    if (t == act - 1) release(&op_empty[k_op % C::SLOTS]);
-                } else {
-                    release(&o_full[t]);
+        uint32_t v_slot = 1, v_phase = 0, k_slot = 2, k_phase = 0;  // of V_j and K_j+1: operands 2j + 1, 2j + 2
+        for (int j = 0; j < n; ++j) {
+            const bool more = j + 1 < n;
+            if (!wait(&op_full[v_slot], v_phase)) break;
+            if (more && !wait(&op_full[k_slot], k_phase)) break;
+            if (!wait(&p_full[0], j & 1)) break;
+            if (elect_one()) {
+                values(0, v_slot, j > 0);
+                if (!two) mma_commit(&op_empty[v_slot]);
+                if (more) scores(0, k_slot);
+                else mma_commit(&o_full[0]);
+                if (more && !two) mma_commit(&op_empty[k_slot]);
+            }
+            __syncwarp();
+            if (two) {
+                if (!wait(&p_full[1], j & 1)) break;
+                if (elect_one()) {
+                    values(1, v_slot, j > 0);
+                    mma_commit(&op_empty[v_slot]);
+                    if (more) scores(1, k_slot);
+                    else mma_commit(&o_full[1]);
+                    if (more) mma_commit(&op_empty[k_slot]);
                 }
+                __syncwarp();
             }
+            v_slot += 2;
+            if (v_slot >= C::SLOTS) v_slot -= C::SLOTS, v_phase ^= 1u;
+            k_slot += 2;
+            if (k_slot >= C::SLOTS) k_slot -= C::SLOTS, k_phase ^= 1u;
         }
-        if (!ok) {  // let what was issued end before the tensor memory is given up
-            release(drain);
+        if (!ok && lane == 0) {  // let what was issued end before the tensor memory is given up
+            mma_commit(drain);
             mbar_wait_drain(drain, 0);
         }
-    } else if (warp == 13) {
+        __syncwarp();
+      } else if (warp == 17) {
         // ---- loader ---------------------------------------------------------------------------
         bool ok = true;
-        int j = 0;
+        int j = 0, next = prompt_look(a, u, u.t0);
         for (; j < tiles && ok; ++j) {
             const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
-            int page;
-            const uint32_t pages = prompt_pages(a, u, tok0, &page);
+            const int page = next;
+            const uint32_t pages = prompt_pages(a, page);
+            next = prompt_look(a, u, u.t0 + j + 1);
             const int st = j % C::NR;
             ok = j < C::NR || mbar_wait(&raw_empty[st], (j / C::NR - 1) & 1, abort);
             ok = __all_sync(0xFFFFFFFFu, ok);
@@ -622,11 +690,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         }
         if (!ok && lane == 0)  // copies in flight end before the memory is given up
             for (int k = max(0, j - C::NR); k < j; ++k) mbar_wait_drain(&raw_full[k % C::NR], (k / C::NR) & 1);
+      }
     }
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         tc_fence_after();
         tmem_relinquish();
         tmem_dealloc(tmem, 512);
