@@ -244,24 +244,24 @@ cudaError_t run_step(const Kv4Attn& a, cudaStream_t st) {
 }
 
 template <int D, bool BF16>
-cudaError_t run_prompt(const Kv4Attn& a, cudaStream_t st) {
+cudaError_t run_prompt(const Kv4Attn& a, int sms, cudaStream_t st) {
     using C = PromptCfg<D>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = prepare_kernel(k_kv4_prompt<C, BF16>, C::SMEM, C::REGS, done);
     if (e != cudaSuccess) return e;
-    const unsigned units = static_cast<unsigned>(a.rows.batch) * a.cache.heads * a.prompt_tiles;
-    e = launch_early(k_kv4_prompt<C, BF16>, dim3(units * a.prompt_splits), kPromptThreads, C::SMEM, st, a);
+    const int ctas = std::min(a.prompt_units * a.prompt_splits, sms);
+    e = launch_early(k_kv4_prompt<C, BF16>, dim3(ctas), kPromptThreads, C::SMEM, st, a);
     if (e != cudaSuccess || a.prompt_splits == 1) return e;
-    k_kv4_prompt_join<C, BF16><<<dim3(units, kPromptRows / 32), 256, 0, st>>>(a);
+    k_kv4_prompt_join<C, BF16><<<dim3(a.prompt_units, kPromptRows / 32), 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 
 template <int D, bool BF16>
-cudaError_t run_attention(const Kv4Attn& a, int nt, cudaStream_t st) {
+cudaError_t run_attention(const Kv4Attn& a, int nt, int sms, cudaStream_t st) {
     if (nt == 1) return run_step<D, 1, BF16>(a, st);
     if (nt == 2) return run_step<D, 2, BF16>(a, st);
     const cudaError_t e = run_step<D, 4, BF16>(a, st);
-    return e == cudaSuccess && a.prompt_tiles ? run_prompt<D, BF16>(a, st) : e;
+    return e == cudaSuccess && a.prompt_tiles ? run_prompt<D, BF16>(a, sms, st) : e;
 }
 
 tb_status check_heads(const tb_kv4_cache* c, int q_heads, int max_rows, int max_len) {
@@ -369,12 +369,14 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     a.prompt_ws = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.step_bytes);
     a.prompt_tiles = p.prompt_tiles;
     a.prompt_splits = p.splits;
-    if (static_cast<long long>(a.rows.batch) * a.cache.heads * std::max(p.prompt_tiles, 1) * p.splits > 0x3FFFFFFFll)
+    const long long units = static_cast<long long>(a.rows.batch) * a.cache.heads * std::max(p.prompt_tiles, 1);
+    if (units * p.splits > 0x3FFFFFFFll)
         return refuse(TB_ERR_SHAPE, "batch * kv_heads * row tiles must stay below 2^30");
+    a.prompt_units = static_cast<int>(units);
     const bool bf16 = fmt == TB_FMT_BF16;
     cudaError_t e;
-    if (a.cache.dim == 128) e = bf16 ? run_attention<128, true>(a, p.nt, stream) : run_attention<128, false>(a, p.nt, stream);
-    else e = bf16 ? run_attention<64, true>(a, p.nt, stream) : run_attention<64, false>(a, p.nt, stream);
+    if (a.cache.dim == 128) e = bf16 ? run_attention<128, true>(a, p.nt, sms, stream) : run_attention<128, false>(a, p.nt, sms, stream);
+    else e = bf16 ? run_attention<64, true>(a, p.nt, sms, stream) : run_attention<64, false>(a, p.nt, sms, stream);
     return launched(e);
 }
 

@@ -1,7 +1,9 @@
 // kv4_prompt_kernel.cuh -- attention of many rows per sequence (a prompt, or a
 // chunk of one) over the block-scaled FP4 cache, on tcgen05.
 //
-// A CTA owns 256 packed rows (token, head of one KV head's group) as two tiles
+// The kernel is persistent: a CTA takes an item of each round, and what loads
+// and decodes goes on into the next one while the last rows are finished.
+// An item is 256 packed rows (token, head of one KV head's group) as two tiles
 // of 128 and runs over their visible tokens in tiles of 128:
 //   S_t = Q_t K^T     tcgen05.mma, both operands in shared memory, S_t in TMEM
 //   P_t = 2^(S_t - m) one thread per row, S_t read from and P_t (FP16) written
@@ -59,6 +61,13 @@ struct PromptCfg {
     static constexpr int SLOT_FLOATS = kPromptRows * (D + 2);
 };
 
+// The CTA's item of round r: there and back through the items, which come
+// largest first, so that the sums are alike.
+__device__ __forceinline__ int prompt_item(int r) {
+    return r * static_cast<int>(gridDim.x) +
+           static_cast<int>(r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 // Low word of the descriptor of an N-major operand tile (V as [token][d]): 64
 // values of N are a 128-byte row, 8 rows of K an atom of 1024 bytes (the stride
 // byte offset, in the high word), 64 more values of N a panel (the leading byte
@@ -74,8 +83,8 @@ __device__ __forceinline__ bool prompt_takes(const Kv4Attn& a, const Kv4Seq& q) 
     return static_cast<long long>(q.n) * a.group > kStepRowsMost;
 }
 
-// A CTA's unit: which rows of which sequence and head, and its share of their
-// tiles of tokens.
+// An item of work: some rows of a sequence and head, and a share of their
+// tiles of tokens (t0 == t1: nothing to do).
 struct PromptUnit {
     Kv4Seq q;
     Kv4Span span;
@@ -85,8 +94,13 @@ struct PromptUnit {
     bool any;
 };
 
-__device__ __forceinline__ PromptUnit prompt_unit(const Kv4Attn& a, int unit, int split) {
+__device__ __forceinline__ PromptUnit prompt_unit(const Kv4Attn& a, int item) {
     PromptUnit u;
+    int unit = item, split = 0;
+    if (a.prompt_splits > 1) {
+        unit = item / a.prompt_splits;
+        split = item - unit * a.prompt_splits;
+    }
     // The last row tiles see the most tokens: they come first.
     const int per_tile = a.rows.batch * a.cache.heads;
     const int tile = a.prompt_tiles - 1 - unit / per_tile;
@@ -96,17 +110,17 @@ __device__ __forceinline__ PromptUnit prompt_unit(const Kv4Attn& a, int unit, in
     u.q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[u.b], a.rows.cu[u.b + 1], a.rows.lens[u.b]);
     u.row_base = tile * kPromptRows;
     u.row_count = min(kPromptRows, u.q.n * a.group - u.row_base);
+    u.t0 = u.t1 = 0;
     u.any = prompt_takes(a, u.q) && u.row_count > 0;
     if (!u.any) return u;
     u.first_pos = u.q.pos0 + u.row_base / a.group;
     u.last_pos = u.q.pos0 + (u.row_base + u.row_count - 1) / a.group;
     u.span = kv4_span(u.first_pos, u.last_pos, u.q.len, a.window, a.sinks, 7);
-    const int tiles = kv4_span_chunks(u.span);
-    u.t0 = 0;
-    u.t1 = tiles;
+    u.t1 = kv4_span_chunks(u.span);
     if (a.prompt_splits > 1) {
-        u.t0 = static_cast<int>(static_cast<long long>(tiles) * split / a.prompt_splits);
-        u.t1 = static_cast<int>(static_cast<long long>(tiles) * (split + 1) / a.prompt_splits);
+        const long long tiles = u.t1;
+        u.t0 = static_cast<int>(tiles * split / a.prompt_splits);
+        u.t1 = static_cast<int>(tiles * (split + 1) / a.prompt_splits);
     }
     return u;
 }
@@ -216,50 +230,41 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
     uint64_t* op_full = raw_empty + C::NR;
     uint64_t* op_empty = op_full + C::SLOTS;
     uint64_t* s_full = op_empty + C::SLOTS;
-    uint64_t* p_full = s_full + 2;
-    uint64_t* o_full = p_full + 2;
+    uint64_t* p_full = s_full + 2;           // [tile of rows][half of the tokens]
+    uint64_t* pv_half = p_full + 4;          // P V of the first half has ended
+    uint64_t* o_full = pv_half + 2;
     uint64_t* q_full = o_full + 2;
     uint64_t* drain = q_full + 2;
     uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-    volatile int* nan_seen = abort + 1;
+    volatile int* nan_seen = abort + 1;  // [round & 3]: the item whose V had a NaN block left out
     float* q_scale = reinterpret_cast<float*>(smem + C::OFF_QSCALE);  // score -> log2 units, per row
 
     // A value that a shuffle or a vote gives is the same in the whole warp for
     // the compiler too, which then keeps what follows from it in uniform
     // registers: MMAs are issued from those.
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid / 32, 0), lane = tid & 31;
-    const int unit = blockIdx.x / a.prompt_splits, split = blockIdx.x - unit * a.prompt_splits;
-    const PromptUnit u = prompt_unit(a, unit, split);
-    const int tiles = u.any ? u.t1 - u.t0 : 0;
-    if (tiles == 0) {
-        grid_dep_wait();  // this grid's end implies the step kernel's
-        return;
-    }
-    const int act = u.row_count > 128 ? 2 : 1;  // tiles of rows in use
-
     if (tid == 0) {
         for (int i = 0; i < C::NR; ++i) {
             mbar_init(&raw_full[i], 1);
             mbar_init(&raw_empty[i], 8);
         }
         for (int i = 0; i < C::SLOTS; ++i) {
-            mbar_init(&op_full[i], 4);
+            mbar_init(&op_full[i], 8);
             mbar_init(&op_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[2 * i], 4);
+            mbar_init(&p_full[2 * i + 1], 4);
+            mbar_init(&pv_half[i], 1);
             mbar_init(&o_full[i], 1);
             mbar_init(&q_full[i], 4);
         }
         mbar_init(drain, 1);
         fence_barrier_init();
         *abort = 0;
-        *nan_seen = 0;
-        if (u.q.bad) atomicOr(&g_tb_device_error, kErrPage);
-        if (static_cast<long long>(u.q.n) * a.group > static_cast<long long>(a.prompt_tiles) * kPromptRows)
-            atomicOr(&g_tb_device_error, kErrRows);
+        for (int i = 0; i < 4; ++i) nan_seen[i] = -1;
     }
     if (warp == 16) tmem_alloc(tmem_ptr, 512);
     tc_fence_before();
@@ -267,6 +272,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
     tc_fence_after();
     const uint32_t tmem = *tmem_ptr;
 
+    const int items = a.prompt_units * a.prompt_splits;
+    const int rounds = (items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
     const int gshift = a.cache.page_shift < 7 ? a.cache.page_shift : 7;
     const uint32_t gtok = 1u << gshift;
     const uint32_t at_ks = gtok * (D / 2), at_vc = at_ks + gtok * (D / 16), at_vs = at_vc + gtok * (D / 2);
@@ -276,7 +283,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         reg_inc<C::REGS_SOFTMAX>();
         // ---- softmax: thread = row ----------------------------------------------------
         const int t = warp / 4, r = tid & 127;
-        if (t < act) {
+        const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane offset 32 * (warp % 4)
+        const uint32_t s_tmem = tmem + quarter + t * C::S_COLS;
+        const uint32_t o_tmem = tmem + quarter + C::O_COL + t * D;
+        uint32_t s_phase = 0, o_phase = 0;
+        bool ok = true;
+        for (int round = 0; round < rounds && ok; ++round) {
+            const int item = prompt_item(round);
+            if (item >= items) break;  // only in the last round
+            const PromptUnit u = prompt_unit(a, item);
+            if (u.t0 == u.t1 || u.row_count <= t * 128) continue;
             const int row = u.row_base + t * 128 + r;
             const bool valid = t * 128 + r < u.row_count;
             const int i = row / a.group;
@@ -288,17 +304,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                 constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
                 const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
                 const int k = lane % LANES;  // 16-byte chunk of the row
+                const int r0 = t * 128 + (warp & 3) * 32 + lane / LANES;
+                int to = (u.row_base + r0) / a.group, head = (u.row_base + r0) - to * a.group;  // of the lane's row
+                const int to_step = AT_ONCE / a.group, head_step = AT_ONCE - to_step * a.group;
+                const uint16_t* src = static_cast<const uint16_t*>(a.q) + u.q.first * a.q_stride +
+                                      static_cast<long long>(u.head) * a.group * D + 8 * k;
                 uint4 v[32 / AT_ONCE];
 #pragma unroll
                 for (int x = 0; x < 32 / AT_ONCE; ++x) {
-                    const int rr = (warp & 3) * 32 + x * AT_ONCE + lane / LANES;
                     v[x] = make_uint4(0u, 0u, 0u, 0u);
-                    if (t * 128 + rr < u.row_count) {
-                        const int ro = u.row_base + t * 128 + rr, to = ro / a.group;
-                        v[x] = *reinterpret_cast<const uint4*>(
-                            static_cast<const uint16_t*>(a.q) + (u.q.first + to) * a.q_stride +
-                            static_cast<long long>(u.head * a.group + ro - to * a.group) * D + 8 * k);
-                    }
+                    if (r0 + x * AT_ONCE < u.row_count)
+                        v[x] = *reinterpret_cast<const uint4*>(src + to * a.q_stride + head * D);
+                    to += to_step;
+                    head += head_step;
+                    if (head >= a.group) head -= a.group, ++to;
                 }
                 uint8_t* q_tile = smem + t * C::OPERAND;
 #pragma unroll
@@ -333,17 +352,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             }
             const float f = q_scale[t * 128 + r];  // written by this warp
 
-            const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane offset 32 * (warp % 4)
-            const uint32_t s_tmem = tmem + quarter + t * C::S_COLS;
-            const uint32_t o_tmem = tmem + quarter + C::O_COL + t * D;
             float m = kNoMax, l = 0.0f;
-            bool ok = true;
             int page = prompt_look(a, u, u.t0);
-            for (int j = 0; j < tiles && ok; ++j) {
-                const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
+            for (int j = u.t0; j < u.t1; ++j) {
+                const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
                 const uint32_t pages = prompt_pages(a, page);
                 const bool open = prompt_open(a, u, tok0, pages);
-                page = prompt_look(a, u, u.t0 + j + 1);
+                page = prompt_look(a, u, j + 1);
                 uint32_t mask[4];
                 if (!open) {
 #pragma unroll
@@ -361,8 +376,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                         mask[c] = w & there;
                     }
                 }
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[t], j & 1, abort));
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[t], s_phase, abort));
                 if (!ok) break;
+                s_phase ^= 1u;
                 tc_fence_after();  // S_t is there, and O_t at rest: its last P V came before
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -372,8 +388,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     float sum;
                     float top = open ? prompt_pass<false>(s_half, f, m, m0, m1, p, &sum)
                                      : prompt_pass<true>(s_half, f, m, m0, m1, p, &sum);
-                    // The first half keeps P below 2^8, the second below 2^15:
-                    // moving m there also means P of the first half again.
+                    // The first half keeps P below 2^8, the second below 2^15,
+                    // since moving m there waits for the first half's P V.
                     if (__any_sync(0xFFFFFFFFu, top > (half == 0 ? 8.0f : 15.0f))) {
                         // The row's largest score, found anew: s f - m has lost
                         // it where m was kNoMax.  m stays a whole number, so
@@ -385,20 +401,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                         l *= scale;
                         if (open) prompt_pass<false>(s_half, f, m, m0, m1, p, &sum);
                         else prompt_pass<true>(s_half, f, m, m0, m1, p, &sum);
-                        if (half == 1) {
-                            const uint32_t by = pack_half2(scale, scale);
-                            tmem_wait_st();
-#pragma unroll 1
-                            for (int c = 0; c < 32; c += 16) {
-                                uint32_t o[16];
-                                tmem_ld_32x32b_x16(s_tmem + c, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int k = 0; k < 16; ++k) o[k] = hmul2(o[k], by);
-                                tmem_st_32x32b_x16(s_tmem + c, o);
-                            }
+                        if (half == 1) {  // O at rest again: P V of the first half has ended
+                            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&pv_half[t], s_phase ^ 1u, abort));
+                            tc_fence_after();
                         }
-                        if (j > 0) {
+                        if (half == 1 || j > u.t0) {
 #pragma unroll 1
                             for (int c = 0; c < D; c += 16) {
                                 uint32_t o[16];
@@ -412,20 +419,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     }
                     l += sum;
                     tmem_st_32x32b_x32(s_tmem + 32 * half, p);  // over scores that have been read
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t]);
             }
 
             // ---- the rows' result --------------------------------------------------------
-            ok = mbar_wait(&o_full[t], 0, abort);
-            named_bar_sync(1, 256 + 128 * act);  // the decode warps have recorded their NaN blocks
-            if (__all_sync(0xFFFFFFFFu, ok)) {
+            ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&o_full[t], o_phase, abort));
+            o_phase ^= 1u;
+            if (ok) {
                 tc_fence_after();
                 uint32_t nan_blocks = 0;
-                if (*nan_seen && valid) {
+                if (nan_seen[round & 3] == item && valid) {
                     // Rare: look at every block of V that was left out of a
                     // partly visible tile, and put a NaN where this row sees it.
                     for (int j = u.t0; j < u.t1; ++j) {
@@ -445,7 +452,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     }
                 }
                 const bool partial = a.prompt_splits > 1;
-                float* slot = a.prompt_ws + static_cast<size_t>(blockIdx.x) * C::SLOT_FLOATS;
+                float* slot = a.prompt_ws + static_cast<size_t>(item) * C::SLOT_FLOATS;
                 const float g = l == 0.0f ? 0.0f : a.cache.v_scale / l;
                 uint16_t* dst = static_cast<uint16_t*>(a.out) + (u.q.first + i) * a.out_stride +
                                 static_cast<long long>(h) * D;
@@ -489,86 +496,85 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     a.lse[static_cast<long long>(u.q.first + i) * a.q_heads + h] =
                         l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                 }
+                tc_fence_before();  // O has been read before the next unit's P is announced
             }
         }
     } else if (warp < 16) {
         reg_dec<C::REGS_DECODE>();
-        // ---- decode: thread = token of the tile; four warps for K, four for V -------------
-        const int kv = (warp - 8) / 4;
-        const uint32_t tok = static_cast<uint32_t>(tid & 127);
+        // ---- decode: thread = half of a token's values, K tile and V tile in turn ---------
+        const uint32_t tok = static_cast<uint32_t>(tid & 127), half = (warp - 8) / 4;
         const uint32_t g0 = (tok >> gshift) * gbytes, place = tok & (gtok - 1u);
+        constexpr int PARTS = D / 64;  // 16-byte parts of the thread's codes: 32 values, two scales each
+        int rs = 0, slot = 0;
+        uint32_t r_phase = 0, op_phase = 1;  // of the empty slot: the first round passes at once
         bool ok = true;
-        int page = prompt_look(a, u, u.t0);
-        for (int j = 0; j < tiles && ok; ++j) {
-            const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
-            const uint32_t pages = prompt_pages(a, page);
-            const bool open = prompt_open(a, u, tok0, pages);
-            page = prompt_look(a, u, u.t0 + j + 1);
-            const bool there = ((pages >> (tok >> gshift)) & 1u) && tok0 + static_cast<int>(tok) < u.q.len;
-            const int st = j % C::NR;
-            ok = mbar_wait(&raw_full[st], (j / C::NR) & 1, abort);
-            const uint32_t n_op = 2 * j + kv;  // K_0, V_0, K_1, ... take the slots in turn
-            const int slot = n_op % C::SLOTS;
-            ok = ok && (n_op < C::SLOTS || mbar_wait(&op_empty[slot], (n_op / C::SLOTS - 1) & 1, abort));
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            const uint8_t* raw = smem + C::OFF_RAW + st * C::RAW + g0;
-            {
-                uint8_t* dst = smem + C::OFF_SLOT + slot * C::OPERAND + tok * 128;
-                const uint8_t* codes = raw + (kv ? at_vc : 0u) + place * (D / 2);
-                const uint8_t* scales = raw + (kv ? at_vs : at_ks) + place * (D / 16);
-                uint32_t sc[D / 64];
-                if constexpr (D == 128) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(scales);
-                    sc[0] = v.x;
-                    sc[1] = v.y;
-                } else {
-                    sc[0] = *reinterpret_cast<const uint32_t*>(scales);
-                }
+        for (int round = 0; round < rounds && ok; ++round) {
+            const int item = prompt_item(round);
+            if (item >= items) break;  // only in the last round
+            const PromptUnit u = prompt_unit(a, item);
+            int page = prompt_look(a, u, u.t0);
+            for (int j = u.t0; j < u.t1; ++j) {
+                const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
+                const uint32_t pages = prompt_pages(a, page);
+                const bool open = prompt_open(a, u, tok0, pages);
+                page = prompt_look(a, u, j + 1);
+                const bool there = ((pages >> (tok >> gshift)) & 1u) && tok0 + static_cast<int>(tok) < u.q.len;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&raw_full[rs], r_phase, abort));
+                if (!ok) break;
+                const uint8_t* raw = smem + C::OFF_RAW + rs * C::RAW + g0;
+#pragma unroll 1
+                for (int kv = 0; kv < 2; ++kv) {
+                    const uint8_t* codes = raw + (kv ? at_vc : 0u) + place * (D / 2) + half * (D / 4);
+                    const uint8_t* scales = raw + (kv ? at_vs : at_ks) + place * (D / 16) + half * (D / 32);
+                    uint4 v[PARTS];
+                    // Lanes start at different parts, so that the writes of a
+                    // quarter warp fall into different banks.
 #pragma unroll
-                for (int x = 0; x < D / 64; ++x) {
-                    if (!there) sc[x] = 0u;
-                    if (kv && !open && e4m3_nan_bits(sc[x])) {
+                    for (int x = 0; x < PARTS; ++x)
+                        v[x] = *reinterpret_cast<const uint4*>(codes + 16 * ((x + (tok >> 1)) & (PARTS - 1)));
+                    uint32_t sc;
+                    if constexpr (D == 128) sc = *reinterpret_cast<const uint32_t*>(scales);
+                    else sc = *reinterpret_cast<const uint16_t*>(scales);
+                    if (!there) sc = 0u;
+                    if (kv && !open && e4m3_nan_bits(sc)) {
                         // A NaN block that some row may not see: out of the
                         // product, and into the rows that see it at the end.
-                        *nan_seen = 1;
-                        const uint32_t n = e4m3_nan_bits(sc[x]) >> 7;  // 1 in the low bit of NaN bytes
-                        sc[x] &= ~(n * 0xFFu);
+                        nan_seen[round & 3] = item;
+                        __threadfence_block();
+                        sc &= ~((e4m3_nan_bits(sc) >> 7) * 0xFFu);
                     }
-                }
-                // Lanes start at different 16-byte parts of their rows, so that
-                // neither the reads nor the writes of a quarter warp share a bank.
-                constexpr int PARTS = D / 32;
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(&op_empty[slot], op_phase, abort));
+                    if (!ok) break;
+                    uint8_t* dst = smem + C::OFF_SLOT + slot * C::OPERAND + tok * 128;
 #pragma unroll
-                for (int x = 0; x < PARTS; ++x) {
-                    const uint32_t part = (x + (tok >> 1)) & (PARTS - 1);
-                    const uint4 v = *reinterpret_cast<const uint4*>(codes + 16 * part);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                    uint32_t s2;  // the part's two scale bytes
-                    if constexpr (D == 128) s2 = (part & 2u ? sc[1] : sc[0]) >> (16 * (part & 1u));
-                    else s2 = sc[0] >> (16 * part);
-                    const uint32_t ss = cvt_e4m3x2(static_cast<uint16_t>(s2));
-                    const uint32_t sa = prmt(ss, 0u, 0x1010u), sb = prmt(ss, 0u, 0x3232u);
+                    for (int x = 0; x < PARTS; ++x) {
+                        const uint32_t part = (x + (tok >> 1)) & (PARTS - 1);
+                        const uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+                        const uint32_t ss = cvt_e4m3x2(static_cast<uint16_t>(sc >> (16 * part)));
+                        const uint32_t sa = prmt(ss, 0u, 0x1010u), sb = prmt(ss, 0u, 0x3232u);
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        uint32_t o[4];
-                        cvt_e2m1x2_x4(w[y], o);
+                        for (int y = 0; y < 4; ++y) {
+                            uint32_t o[4];
+                            cvt_e2m1x2_x4(w[y], o);
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) o[z] = hmul2(o[z], y < 2 ? sa : sb);
-                        const uint32_t chunk = 4 * part + y;  // 16-byte chunk of the decoded row
-                        *reinterpret_cast<uint4*>(dst + (chunk >> 3) * C::PANEL + (((chunk & 7u) ^ (tok & 7u)) << 4)) =
-                            make_uint4(o[0], o[1], o[2], o[3]);
+                            for (int z = 0; z < 4; ++z) o[z] = hmul2(o[z], y < 2 ? sa : sb);
+                            const uint32_t chunk = (D / 16) * half + 4 * part + y;  // 16-byte chunk of the decoded row
+                            *reinterpret_cast<uint4*>(dst + (chunk >> 3) * C::PANEL + (((chunk & 7u) ^ (tok & 7u)) << 4)) =
+                                make_uint4(o[0], o[1], o[2], o[3]);
+                        }
                     }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&op_full[slot]);
+                        if (kv) mbar_arrive(&raw_empty[rs]);
+                    }
+                    if (++slot == C::SLOTS) slot = 0, op_phase ^= 1u;
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&op_full[slot]);
-                    mbar_arrive(&raw_empty[st]);
-                }
+                if (!ok) break;
+                if (++rs == C::NR) rs = 0, r_phase ^= 1u;
             }
         }
-        named_bar_sync(1, 256 + 128 * act);
     } else {
       reg_dec<C::REGS_REST>();
       if (warp == 16) {
@@ -578,8 +584,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         constexpr uint32_t idesc_o = idesc_make(0, 0, 128, D) | (1u << 16);  // V is N-major
         const uint32_t q_lo = sdesc_lo(smem_addr(smem));
         const uint32_t k_lo = sdesc_lo(smem_addr(smem + C::OFF_SLOT)), v_lo = sdesc_v_lo<C>(smem_addr(smem + C::OFF_SLOT));
-        const int n = __reduce_max_sync(0xFFFFFFFFu, tiles);
-        const bool two = __any_sync(0xFFFFFFFFu, act == 2);
         bool ok = __all_sync(0xFFFFFFFFu, tmem == 0u);
         if (!ok && lane == 0) {
             atomicOr(&g_tb_device_error, kErrTimeout);
@@ -600,52 +604,92 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             }
             mma_commit(&s_full[t]);
         };
-        auto values = [&](int t, uint32_t slot, uint32_t accumulate) {
+        // O_t += P_t V of half the tokens.
+        auto values = [&](int t, uint32_t slot, int half, uint32_t accumulate) {
             const uint32_t vl = v_lo + slot * (C::OPERAND >> 4);
 #pragma unroll
-            for (int k = 0; k < kPromptTile / 16; ++k)
+            for (int x = 0; x < kPromptTile / 32; ++x) {
+                const int k = half * (kPromptTile / 32) + x;
                 mma_f16_ts(C::O_COL + t * D, t * C::S_COLS + 8 * k, sdesc_make(vl + k * (2048 >> 4)), idesc_o,
-                           k > 0 ? 1u : accumulate);
+                           x > 0 ? 1u : accumulate);
+            }
         };
-        wait(&q_full[0], 0);
-        if (two) wait(&q_full[1], 0);
-        if (wait(&op_full[0], 0)) {
-            if (elect_one()) {
-                scores(0, 0);
-                if (two) scores(1, 0);
-                mma_commit(&op_empty[0]);
-            }
-            __syncwarp();
-        }
-        uint32_t v_slot = 1, v_phase = 0, k_slot = 2, k_phase = 0;  // of V_j and K_j+1: operands 2j + 1, 2j + 2
-        for (int j = 0; j < n; ++j) {
-            const bool more = j + 1 < n;
-            if (!wait(&op_full[v_slot], v_phase)) break;
-            if (more && !wait(&op_full[k_slot], k_phase)) break;
-            if (!wait(&p_full[0], j & 1)) break;
-            if (elect_one()) {
-                values(0, v_slot, j > 0);
-                if (!two) mma_commit(&op_empty[v_slot]);
-                if (more) scores(0, k_slot);
-                else mma_commit(&o_full[0]);
-                if (more && !two) mma_commit(&op_empty[k_slot]);
-            }
-            __syncwarp();
+        int slot = 0;  // operands take the slots in turn: K_0, V_0, K_1, V_1, ...
+        uint32_t op_phase = 0, p_phase0 = 0, p_phase1 = 0, q_phase0 = 0, q_phase1 = 0;
+        auto next = [&]() {
+            if (++slot == C::SLOTS) slot = 0, op_phase ^= 1u;
+        };
+        for (int round = 0; round < rounds && ok; ++round) {
+            const int item = prompt_item(round);
+            if (item >= items) break;  // only in the last round
+            const PromptUnit u = prompt_unit(a, item);
+            const int n = __reduce_max_sync(0xFFFFFFFFu, u.t1 - u.t0);
+            if (n == 0) continue;
+            const bool two = __any_sync(0xFFFFFFFFu, u.row_count > 128);
+            if (!wait(&q_full[0], q_phase0)) break;
+            q_phase0 ^= 1u;
             if (two) {
-                if (!wait(&p_full[1], j & 1)) break;
+                if (!wait(&q_full[1], q_phase1)) break;
+                q_phase1 ^= 1u;
+            }
+            if (!wait(&op_full[slot], op_phase)) break;
+            if (elect_one()) {
+                scores(0, slot);
+                if (two) scores(1, slot);
+                mma_commit(&op_empty[slot]);
+            }
+            __syncwarp();
+            next();
+            for (int j = 0; j < n; ++j) {
+                const bool more = j + 1 < n;
+                const int v_slot = slot;
+                if (!wait(&op_full[slot], op_phase)) break;
+                next();
+                if (!wait(&p_full[0], p_phase0)) break;
                 if (elect_one()) {
-                    values(1, v_slot, j > 0);
-                    mma_commit(&op_empty[v_slot]);
-                    if (more) scores(1, k_slot);
-                    else mma_commit(&o_full[1]);
-                    if (more) mma_commit(&op_empty[k_slot]);
+                    values(0, v_slot, 0, j > 0);
+                    mma_commit(&pv_half[0]);
                 }
                 __syncwarp();
+                if (!wait(&p_full[1], p_phase0)) break;
+                p_phase0 ^= 1u;
+                if (elect_one()) {
+                    values(0, v_slot, 1, 1u);
+                    if (!two) mma_commit(&op_empty[v_slot]);
+                    if (!more) mma_commit(&o_full[0]);
+                }
+                __syncwarp();
+                if (more) {
+                    if (!wait(&op_full[slot], op_phase)) break;
+                    if (elect_one()) {
+                        scores(0, slot);
+                        if (!two) mma_commit(&op_empty[slot]);
+                    }
+                    __syncwarp();
+                }
+                if (two) {
+                    if (!wait(&p_full[2], p_phase1)) break;
+                    if (elect_one()) {
+                        values(1, v_slot, 0, j > 0);
+                        mma_commit(&pv_half[1]);
+                    }
+                    __syncwarp();
+                    if (!wait(&p_full[3], p_phase1)) break;
+                    p_phase1 ^= 1u;
+                    if (elect_one()) {
+                        values(1, v_slot, 1, 1u);
+                        mma_commit(&op_empty[v_slot]);
+                        if (more) {
+                            scores(1, slot);
+                            mma_commit(&op_empty[slot]);
+                        } else {
+                            mma_commit(&o_full[1]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (more) next();
             }
-            v_slot += 2;
-            if (v_slot >= C::SLOTS) v_slot -= C::SLOTS, v_phase ^= 1u;
-            k_slot += 2;
-            if (k_slot >= C::SLOTS) k_slot -= C::SLOTS, k_phase ^= 1u;
         }
         if (!ok && lane == 0) {  // let what was issued end before the tensor memory is given up
             mma_commit(drain);
@@ -654,42 +698,57 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         __syncwarp();
       } else if (warp == 17) {
         // ---- loader ---------------------------------------------------------------------------
+        int rs = 0;
+        uint32_t r_phase = 1, filled = 0;  // of the empty stage: the first round passes at once
         bool ok = true;
-        int j = 0, next = prompt_look(a, u, u.t0);
-        for (; j < tiles && ok; ++j) {
-            const int tok0 = kv4_span_chunk(u.span, u.t0 + j) * kPromptTile;
-            const int page = next;
-            const uint32_t pages = prompt_pages(a, page);
-            next = prompt_look(a, u, u.t0 + j + 1);
-            const int st = j % C::NR;
-            ok = j < C::NR || mbar_wait(&raw_empty[st], (j / C::NR - 1) & 1, abort);
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            uint8_t* dst = smem + C::OFF_RAW + st * C::RAW;
-            const int want = min(kPromptTile, u.q.len - tok0);  // tokens that should have pages
-            const bool mine = (pages >> lane) & 1u;
-            if ((lane << gshift) < want && !mine) atomicOr(&g_tb_device_error, kErrPage);
-            if (lane == 0) mbar_arrive_expect_tx(&raw_full[st], __popc(pages) * gbytes);
-            __syncwarp();
-            if (mine) {
-                const uint8_t* src = a.cache.data + kv4_block_offset(a.cache, page, u.head);
-                uint8_t* to = dst + lane * gbytes;
-                if (a.cache.page_shift <= 7) {
-                    bulk_load(to, src, gbytes, &raw_full[st]);
-                } else {  // a tile of a larger page, part by part (lane 0 alone)
-                    const uint32_t place_in_page = static_cast<uint32_t>(tok0) & ((1u << a.cache.page_shift) - 1u);
-                    const uint32_t codes = kv4_codes_bytes(a.cache), scales = kv4_scales_bytes(a.cache);
-                    bulk_load(to, src + place_in_page * (D / 2), at_ks, &raw_full[st]);
-                    bulk_load(to + at_ks, src + codes + place_in_page * (D / 16), gtok * (D / 16), &raw_full[st]);
-                    src += codes + scales;
-                    bulk_load(to + at_vc, src + place_in_page * (D / 2), at_ks, &raw_full[st]);
-                    bulk_load(to + at_vs, src + codes + place_in_page * (D / 16), gtok * (D / 16), &raw_full[st]);
-                }
+        for (int round = 0; round < rounds && ok; ++round) {
+            const int item = prompt_item(round);
+            if (item >= items) break;  // only in the last round
+            const PromptUnit u = prompt_unit(a, item);
+            if (lane == 0 && u.any) {
+                if (u.q.bad) atomicOr(&g_tb_device_error, kErrPage);
+                if (static_cast<long long>(u.q.n) * a.group > static_cast<long long>(a.prompt_tiles) * kPromptRows)
+                    atomicOr(&g_tb_device_error, kErrRows);
             }
-            __syncwarp();
+            int after = prompt_look(a, u, u.t0);
+            for (int j = u.t0; j < u.t1; ++j) {
+                const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
+                const int page = after;
+                const uint32_t pages = prompt_pages(a, page);
+                after = prompt_look(a, u, j + 1);
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&raw_empty[rs], r_phase, abort));
+                if (!ok) break;
+                uint8_t* dst = smem + C::OFF_RAW + rs * C::RAW;
+                const int want = min(kPromptTile, u.q.len - tok0);  // tokens that should have pages
+                const bool mine = (pages >> lane) & 1u;
+                if ((lane << gshift) < want && !mine) atomicOr(&g_tb_device_error, kErrPage);
+                if (lane == 0) mbar_arrive_expect_tx(&raw_full[rs], __popc(pages) * gbytes);
+                __syncwarp();
+                if (mine) {
+                    const uint8_t* src = a.cache.data + kv4_block_offset(a.cache, page, u.head);
+                    uint8_t* to = dst + lane * gbytes;
+                    if (a.cache.page_shift <= 7) {
+                        bulk_load(to, src, gbytes, &raw_full[rs]);
+                    } else {  // a tile of a larger page, part by part (lane 0 alone)
+                        const uint32_t place_in_page = static_cast<uint32_t>(tok0) & ((1u << a.cache.page_shift) - 1u);
+                        const uint32_t codes = kv4_codes_bytes(a.cache), scales = kv4_scales_bytes(a.cache);
+                        bulk_load(to, src + place_in_page * (D / 2), at_ks, &raw_full[rs]);
+                        bulk_load(to + at_ks, src + codes + place_in_page * (D / 16), gtok * (D / 16), &raw_full[rs]);
+                        src += codes + scales;
+                        bulk_load(to + at_vc, src + place_in_page * (D / 2), at_ks, &raw_full[rs]);
+                        bulk_load(to + at_vs, src + codes + place_in_page * (D / 16), gtok * (D / 16), &raw_full[rs]);
+                    }
+                }
+                __syncwarp();
+                ++filled;
+                if (++rs == C::NR) rs = 0, r_phase ^= 1u;
+            }
         }
         if (!ok && lane == 0)  // copies in flight end before the memory is given up
-            for (int k = max(0, j - C::NR); k < j; ++k) mbar_wait_drain(&raw_full[k % C::NR], (k / C::NR) & 1);
+            for (int k = 0; k < C::NR && filled > 0; ++k, --filled) {
+                if (--rs < 0) rs = C::NR - 1, r_phase ^= 1u;
+                mbar_wait_drain(&raw_full[rs], r_phase ^ 1u);
+            }
       }
     }
 
@@ -708,7 +767,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
 template <class C, bool BF16>
 __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4Attn a) {
     constexpr int D = C::D;
-    const PromptUnit u = prompt_unit(a, blockIdx.x, 0);
+    const PromptUnit u = prompt_unit(a, blockIdx.x * a.prompt_splits);
     if (!u.any) return;
     const int tiles = kv4_span_chunks(u.span);
     const int r0 = blockIdx.y * 32, r1 = min(r0 + 32, u.row_count);

@@ -63,6 +63,7 @@ struct Kv4Attn {
     float* prompt_ws;
     int prompt_tiles;              // tiles of 256 packed rows of a sequence at most
     int prompt_splits;             // CTAs that share a prompt unit's tokens
+    int prompt_units;              // sequences * KV heads * prompt_tiles
 };
 
 // Bit of the device error word: a sequence has more rows than max_rows.
