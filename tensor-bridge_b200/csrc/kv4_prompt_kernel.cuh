@@ -220,6 +220,83 @@ __device__ __noinline__ float prompt_top(uint32_t s_tmem, float f, uint32_t mask
     return top;
 }
 
+// Queries of a warp's 32 rows of tile t on their way: D / 8 lanes load a row.
+template <class C>
+struct PromptQ {
+    static constexpr int LANES = C::D / 8, AT_ONCE = 32 / LANES, N = 32 / AT_ONCE;
+    uint4 v[N];
+};
+
+template <class C>
+__device__ __forceinline__ void prompt_q_load(const Kv4Attn& a, const PromptUnit& u, int r0, PromptQ<C>& q) {
+    using Q = PromptQ<C>;
+    const int lane = threadIdx.x & 31, k = lane % Q::LANES;  // 16-byte chunk of the row
+    r0 += lane / Q::LANES;
+    int to = (u.row_base + r0) / a.group, head = (u.row_base + r0) - to * a.group;  // of the lane's row
+    const int to_step = Q::AT_ONCE / a.group, head_step = Q::AT_ONCE - to_step * a.group;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + u.q.first * a.q_stride +
+                          static_cast<long long>(u.head) * a.group * C::D + 8 * k;
+#pragma unroll
+    for (int x = 0; x < Q::N; ++x) {
+        q.v[x] = make_uint4(0u, 0u, 0u, 0u);
+        if (r0 + x * Q::AT_ONCE < u.row_count)
+            q.v[x] = *reinterpret_cast<const uint4*>(src + to * a.q_stride + head * C::D);
+        to += to_step;
+        head += head_step;
+        if (head >= a.group) head -= a.group, ++to;
+    }
+}
+
+// ... and into the tile, pairs swapped; BF16 scaled and the sign of the factor
+// moved as in the step kernel.  `scale` gets the rows' factors.
+template <class C, bool BF16>
+__device__ __forceinline__ void prompt_q_store(const Kv4Attn& a, const PromptQ<C>& q, uint8_t* tile, int r0,
+                                               float* scale) {
+    using Q = PromptQ<C>;
+    const int lane = threadIdx.x & 31, k = lane % Q::LANES;
+    const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int x = 0; x < Q::N; ++x) {
+        const int rr = r0 + x * Q::AT_ONCE + lane / Q::LANES;
+        uint32_t w[4] = {q.v[x].x, q.v[x].y, q.v[x].z, q.v[x].w};
+        float f = fmaxf(fabsf(a.scale_log2), 1e-37f);
+        if constexpr (BF16) {
+            uint32_t e = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e = max(e, max((w[j] >> 7) & 0xFFu, (w[j] >> 23) & 0xFFu));
+#pragma unroll
+            for (int d = 1; d < Q::LANES; d <<= 1) e = max(e, __shfl_xor_sync(0xFFFFFFFFu, e, d));
+            const int kk = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = kk > 120 ? 120 : kk, k2 = kk - k1;
+            const float up = exp2i(k1), up2 = exp2i(k2);
+            f = fmaxf((f * exp2i(-k1)) * exp2i(-k2), 1e-37f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[j] = pack_half2(__uint_as_float(w[j] & 0xFFFF0000u) * up * up2, __uint_as_float(w[j] << 16) * up * up2);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = prmt(w[j], 0u, 0x1032u);
+        }
+        if (k == 0) scale[rr] = f;
+        *reinterpret_cast<uint4*>(tile + (k / 8) * C::PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) =
+            make_uint4(w[0] ^ sign, w[1] ^ sign, w[2] ^ sign, w[3] ^ sign);
+    }
+}
+
+// Where tile t's thread r of an item belongs.
+struct PromptRow {
+    bool valid;
+    int pos, at, head;  // position; row of the caller's arrays; query head
+};
+__device__ __forceinline__ PromptRow prompt_row(const Kv4Attn& a, const PromptUnit& u, int r) {
+    PromptRow p;
+    const int row = u.row_base + r, i = row / a.group;
+    p.valid = r < u.row_count;
+    p.pos = u.q.pos0 + i;
+    p.at = u.q.first + i;
+    p.head = u.head * a.group + row - i * a.group;
+    return p;
+}
+
 template <class C, bool BF16>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn a) {
     constexpr int D = C::D;
@@ -288,70 +365,36 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         const uint32_t o_tmem = tmem + quarter + C::O_COL + t * D;
         uint32_t s_phase = 0, o_phase = 0;
         bool ok = true;
-        for (int round = 0; round < rounds && ok; ++round) {
-            const int item = prompt_item(round);
-            if (item >= items) break;  // only in the last round
-            const PromptUnit u = prompt_unit(a, item);
-            if (u.t0 == u.t1 || u.row_count <= t * 128) continue;
-            const int row = u.row_base + t * 128 + r;
-            const bool valid = t * 128 + r < u.row_count;
-            const int i = row / a.group;
-            const int pos = u.q.pos0 + i;
-            const int h = u.head * a.group + row - i * a.group;
-            // Q into its tile, pairs swapped; BF16 scaled and the sign of the
-            // factor moved as in the step kernel.  D / 8 lanes load a row.
-            {
-                constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
-                const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-                const int k = lane % LANES;  // 16-byte chunk of the row
-                const int r0 = t * 128 + (warp & 3) * 32 + lane / LANES;
-                int to = (u.row_base + r0) / a.group, head = (u.row_base + r0) - to * a.group;  // of the lane's row
-                const int to_step = AT_ONCE / a.group, head_step = AT_ONCE - to_step * a.group;
-                const uint16_t* src = static_cast<const uint16_t*>(a.q) + u.q.first * a.q_stride +
-                                      static_cast<long long>(u.head) * a.group * D + 8 * k;
-                uint4 v[32 / AT_ONCE];
-#pragma unroll
-                for (int x = 0; x < 32 / AT_ONCE; ++x) {
-                    v[x] = make_uint4(0u, 0u, 0u, 0u);
-                    if (r0 + x * AT_ONCE < u.row_count)
-                        v[x] = *reinterpret_cast<const uint4*>(src + to * a.q_stride + head * D);
-                    to += to_step;
-                    head += head_step;
-                    if (head >= a.group) head -= a.group, ++to;
-                }
-                uint8_t* q_tile = smem + t * C::OPERAND;
-#pragma unroll
-                for (int x = 0; x < 32 / AT_ONCE; ++x) {
-                    const int rr = (warp & 3) * 32 + x * AT_ONCE + lane / LANES;
-                    uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
-                    float f = fmaxf(fabsf(a.scale_log2), 1e-37f);
-                    if constexpr (BF16) {
-                        uint32_t e = 0;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e = max(e, max((w[j] >> 7) & 0xFFu, (w[j] >> 23) & 0xFFu));
-#pragma unroll
-                        for (int d = 1; d < LANES; d <<= 1) e = max(e, __shfl_xor_sync(0xFFFFFFFFu, e, d));
-                        const int kk = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = kk > 120 ? 120 : kk, k2 = kk - k1;
-                        const float up = exp2i(k1), up2 = exp2i(k2);
-                        f = fmaxf((f * exp2i(-k1)) * exp2i(-k2), 1e-37f);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            w[j] = pack_half2(__uint_as_float(w[j] & 0xFFFF0000u) * up * up2,
-                                              __uint_as_float(w[j] << 16) * up * up2);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) w[j] = prmt(w[j], 0u, 0x1032u);
-                    }
-                    if (k == 0) q_scale[t * 128 + rr] = f;
-                    *reinterpret_cast<uint4*>(q_tile + (k / 8) * C::PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) =
-                        make_uint4(w[0] ^ sign, w[1] ^ sign, w[2] ^ sign, w[3] ^ sign);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[t]);
+        const int warp_row = (warp & 3) * 32;  // first of the warp's rows in the tile
+        uint8_t* q_tile = smem + t * C::OPERAND;
+        // The next round with rows for this tile, from `round` on.
+        auto find = [&](int round, PromptUnit& u) {
+            for (; round < rounds; ++round) {
+                const int item = prompt_item(round);
+                if (item >= items) return rounds;  // only in the last round
+                u = prompt_unit(a, item);
+                if (u.t0 < u.t1 && u.row_count > t * 128) break;
             }
+            return round;
+        };
+        auto give_q = [&](const PromptQ<C>& q) {
+            prompt_q_store<C, BF16>(a, q, q_tile, warp_row, q_scale + t * 128);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[t]);
+        };
+        PromptUnit u;
+        int round = find(0, u);
+        if (round < rounds) {
+            PromptQ<C> q;
+            prompt_q_load<C>(a, u, t * 128 + warp_row, q);
+            give_q(q);
+        }
+        while (round < rounds && ok) {
+            const int item = prompt_item(round);
+            const PromptRow row = prompt_row(a, u, t * 128 + r);
+            const int pos = row.pos;
             const float f = q_scale[t * 128 + r];  // written by this warp
-
             float m = kNoMax, l = 0.0f;
             int page = prompt_look(a, u, u.t0);
             for (int j = u.t0; j < u.t1; ++j) {
@@ -386,15 +429,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     const uint32_t m0 = open ? 0xFFFFFFFFu : mask[2 * half], m1 = open ? 0xFFFFFFFFu : mask[2 * half + 1];
                     uint32_t p[32];
                     float sum;
-                    float top = open ? prompt_pass<false>(s_half, f, m, m0, m1, p, &sum)
-                                     : prompt_pass<true>(s_half, f, m, m0, m1, p, &sum);
+                    float top = INFINITY;  // the item's first scores only set m
+                    if (half == 1 || j > u.t0)
+                        top = open ? prompt_pass<false>(s_half, f, m, m0, m1, p, &sum)
+                                   : prompt_pass<true>(s_half, f, m, m0, m1, p, &sum);
                     // The first half keeps P below 2^8, the second below 2^15,
                     // since moving m there waits for the first half's P V.
-                    if (__any_sync(0xFFFFFFFFu, top > (half == 0 ? 8.0f : 15.0f))) {
+                    const bool move = top > (half == 0 ? 8.0f : 15.0f);
+                    if (__any_sync(0xFFFFFFFFu, move)) {
                         // The row's largest score, found anew: s f - m has lost
                         // it where m was kNoMax.  m stays a whole number, so
                         // that what is scaled by its steps is not rounded.
-                        const float m_new = fmaxf(m, ceilf(prompt_top(s_half, f, m0, m1)));
+                        const float y = ceilf(prompt_top(s_half, f, m0, m1));
+                        const float m_new = move ? fmaxf(m, y) : m;  // the warp's other rows go through the same values again
                         const float step = m_new - m;
                         const float scale = step < 126.0f ? exp2i(-static_cast<int>(step)) : 0.0f;
                         m = m_new;
@@ -426,78 +473,125 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                 }
             }
 
-            // ---- the rows' result --------------------------------------------------------
+            // ---- the rows' result ----------------------------------------------------------
+            PromptUnit un;
+            const int round_next = find(round + 1, un);
             ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&o_full[t], o_phase, abort));
             o_phase ^= 1u;
-            if (ok) {
-                tc_fence_after();
-                uint32_t nan_blocks = 0;
-                if (nan_seen[round & 3] == item && valid) {
-                    // Rare: look at every block of V that was left out of a
-                    // partly visible tile, and put a NaN where this row sees it.
-                    for (int j = u.t0; j < u.t1; ++j) {
-                        const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
-                        for (int k = 0; k < kPromptTile; ++k) {
-                            const int tok = tok0 + k;
-                            if (tok >= u.q.len || !kv4_sees(pos, tok, a.window, a.sinks)) continue;
-                            const int pg = a.rows.table[static_cast<size_t>(u.b) * a.rows.width +
-                                                        (tok >> a.cache.page_shift)];
-                            if (!kv4_page_ok(a.cache, pg)) continue;
-                            const uint8_t* sc = a.cache.data + kv4_block_offset(a.cache, pg, u.head) +
-                                                2 * kv4_codes_bytes(a.cache) + kv4_scales_bytes(a.cache) +
-                                                (tok & ((1 << a.cache.page_shift) - 1)) * (D / 16);
-                            for (int x = 0; x < D / 16; ++x)
-                                if ((sc[x] & 0x7F) == 0x7F) nan_blocks |= 1u << x;
-                        }
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t nan_blocks = 0;
+            if (nan_seen[round & 3] == item && row.valid) {
+                // Rare: look at every block of V that was left out of a
+                // partly visible tile, and put a NaN where this row sees it.
+                for (int j = u.t0; j < u.t1; ++j) {
+                    const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
+                    for (int k = 0; k < kPromptTile; ++k) {
+                        const int tok = tok0 + k;
+                        if (tok >= u.q.len || !kv4_sees(pos, tok, a.window, a.sinks)) continue;
+                        const int pg = a.rows.table[static_cast<size_t>(u.b) * a.rows.width + (tok >> a.cache.page_shift)];
+                        if (!kv4_page_ok(a.cache, pg)) continue;
+                        const uint8_t* sc = a.cache.data + kv4_block_offset(a.cache, pg, u.head) +
+                                            2 * kv4_codes_bytes(a.cache) + kv4_scales_bytes(a.cache) +
+                                            (tok & ((1 << a.cache.page_shift) - 1)) * (D / 16);
+                        for (int x = 0; x < D / 16; ++x)
+                            if ((sc[x] & 0x7F) == 0x7F) nan_blocks |= 1u << x;
                     }
                 }
-                const bool partial = a.prompt_splits > 1;
-                float* slot = a.prompt_ws + static_cast<size_t>(item) * C::SLOT_FLOATS;
-                const float g = l == 0.0f ? 0.0f : a.cache.v_scale / l;
-                uint16_t* dst = static_cast<uint16_t*>(a.out) + (u.q.first + i) * a.out_stride +
-                                static_cast<long long>(h) * D;
+            }
+            const bool partial = a.prompt_splits > 1;
+            const float g = partial ? 1.0f : l == 0.0f ? 0.0f : a.cache.v_scale / l;
+            // The warp's 32 rows go through its part of the query tile (whose
+            // products have ended), D / 8 chunks of 16 bytes of a row at a time,
+            // chunk x at x ^ (row & 7) of its panel, so that they leave in whole
+            // lines: with a row a thread this took 5 us an item.
+            float* slot = a.prompt_ws + static_cast<size_t>(item) * C::SLOT_FLOATS;
+            uint8_t* stage = q_tile + warp_row * 128;
+            uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(u.head) * a.group * D +
+                            8 * (lane % PromptQ<C>::LANES);
+            const int width = partial ? D / 2 : D;  // columns of a pass
+            for (int col = 0; col < D; col += width) {
+                auto put = [&](int x, uint4 v) {
+                    *reinterpret_cast<uint4*>(stage + (x >> 3) * C::PANEL + lane * 128 + (((x & 7) ^ (lane & 7)) << 4)) = v;
+                };
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld_32x32b_x32(o_tmem + c, o);
+                for (int c = 0; c < width; c += 32) {
+                    uint32_t o[32];  // columns come in swapped pairs
+                    tmem_ld_32x32b_x32(o_tmem + col + c, o);
                     tmem_wait_ld();
-                    if (!valid) continue;
+                    if (nan_blocks) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if ((nan_blocks >> ((c + k) / 16)) & 1u) o[k] = 0x7FC00000u;
+                        for (int k = 0; k < 32; ++k)
+                            if ((nan_blocks >> ((col + c + k) / 16)) & 1u) o[k] = 0x7FC00000u;
+                    }
                     if (partial) {
-                        float* to = slot + (t * 128 + r) * D + c;
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4)
-                            *reinterpret_cast<uint4*>(to + k) = make_uint4(o[k + 1], o[k], o[k + 3], o[k + 2]);
+                        for (int k = 0; k < 8; ++k)
+                            put(c / 4 + k, make_uint4(o[4 * k + 1], o[4 * k], o[4 * k + 3], o[4 * k + 2]));
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
+                        for (int k = 0; k < 4; ++k) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                const float lo = l == 0.0f ? 0.0f : __uint_as_float(o[k + 2 * x + 1]) * g;
-                                const float hi = l == 0.0f ? 0.0f : __uint_as_float(o[k + 2 * x]) * g;
+                            for (int y = 0; y < 4; ++y) {
+                                float lo = __uint_as_float(o[8 * k + 2 * y + 1]) * g;
+                                float hi = __uint_as_float(o[8 * k + 2 * y]) * g;
+                                if (l == 0.0f) lo = hi = 0.0f;
                                 if constexpr (BF16) {
-                                    const __nv_bfloat162 y = __floats2bfloat162_rn(lo, hi);
-                                    w[x] = *reinterpret_cast<const uint32_t*>(&y);
+                                    const __nv_bfloat162 z = __floats2bfloat162_rn(lo, hi);
+                                    w[y] = *reinterpret_cast<const uint32_t*>(&z);
                                 } else {
-                                    w[x] = pack_half2(lo, hi);
+                                    w[y] = pack_half2(lo, hi);
                                 }
                             }
-                            *reinterpret_cast<uint4*>(dst + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+                            put(c / 8 + k, make_uint4(w[0], w[1], w[2], w[3]));
                         }
                     }
                 }
-                if (valid && partial) {
-                    slot[kPromptRows * D + t * 128 + r] = m;
-                    slot[kPromptRows * (D + 1) + t * 128 + r] = l;
-                } else if (valid && a.lse != nullptr) {
-                    a.lse[static_cast<long long>(u.q.first + i) * a.q_heads + h] =
-                        l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                __syncwarp();
+                using Q = PromptQ<C>;
+                const int x = lane % Q::LANES;
+                int rr = lane / Q::LANES;
+                const PromptRow first = prompt_row(a, u, t * 128 + warp_row + rr);
+                int at = first.at, head = first.head - u.head * a.group;
+                const int at_step = Q::AT_ONCE / a.group, head_step = Q::AT_ONCE - at_step * a.group;
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part) {
+                    uint4 v[Q::N / 2];
+#pragma unroll
+                    for (int k = 0; k < Q::N / 2; ++k)
+                        v[k] = *reinterpret_cast<const uint4*>(stage + (x >> 3) * C::PANEL + (rr + k * Q::AT_ONCE) * 128 +
+                                                               (((x & 7) ^ ((rr + k * Q::AT_ONCE) & 7)) << 4));
+#pragma unroll
+                    for (int k = 0; k < Q::N / 2; ++k) {
+                        const int tr = t * 128 + warp_row + rr;
+                        if (tr < u.row_count) {
+                            if (partial)
+                                *reinterpret_cast<uint4*>(slot + tr * D + col + 4 * x) = v[k];
+                            else
+                                *reinterpret_cast<uint4*>(out + at * a.out_stride + head * D) = v[k];
+                        }
+                        rr += Q::AT_ONCE;
+                        at += at_step;
+                        head += head_step;
+                        if (head >= a.group) head -= a.group, ++at;
+                    }
                 }
-                tc_fence_before();  // O has been read before the next unit's P is announced
+                __syncwarp();
             }
+            PromptQ<C> q;
+            if (round_next < rounds) prompt_q_load<C>(a, un, t * 128 + warp_row, q);
+            if (row.valid && partial) {
+                slot[kPromptRows * D + t * 128 + r] = m;
+                slot[kPromptRows * (D + 1) + t * 128 + r] = l;
+            } else if (row.valid && a.lse != nullptr) {
+                a.lse[static_cast<long long>(row.at) * a.q_heads + row.head] =
+                    l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+            }
+            tc_fence_before();  // O has been read before the next item's P is announced
+            if (round_next < rounds) give_q(q);
+            u = un;
+            round = round_next;
         }
     } else if (warp < 16) {
         reg_dec<C::REGS_DECODE>();
