@@ -157,14 +157,14 @@ struct AttnPlan {
 AttnPlan plan_attention(int batch, int heads, int dim, int page_shift, int group, int max_rows, int max_len, int sms) {
     AttnPlan p{};
     const long long rows = static_cast<long long>(max_rows) * group;
-    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
     p.runs = sms * (p.nt == 1 ? 2 : 1);
     // Clusters where they all fit on the GPU at once, a tile of tokens or more
     // to a CTA; 8 rows, 8 KV heads of 128, pages of 16, one sequence of 1000,
     // 4096, 16384 tokens: 7.2, 8.5, 17.3 us against 9.7, 10.4, 17.1 us in runs.
-    p.cluster = std::max(1, std::min(8, (max_len + kStepTile - 1) / kStepTile));
+    p.cluster = std::max(1, std::min(8, (max_len + 255) / 256));
     if (max_len > 16384 || static_cast<long long>(batch) * heads * p.cluster > p.runs) p.cluster = 0;
-    p.min_run = std::max(1, 512 >> step_gran(page_shift));
+    p.min_run = std::max(1, 512 >> step_gran(page_shift, p.nt == 2 ? 7 : 8));
     p.step_bytes = p.cluster ? 0 : static_cast<size_t>(p.runs) * 2 * (8 * p.nt) * (dim + 2) * sizeof(float);
     p.splits = 1;
     p.bytes = p.step_bytes;
@@ -235,8 +235,8 @@ cudaError_t run_step(const Kv4Attn& a, cudaStream_t st) {
     cudaError_t e = prepare_kernel(k_kv4_step<C, BF16>, C::SMEM, C::REGS, done);
     if (e != cudaSuccess) return e;
     const unsigned units = static_cast<unsigned>(a.rows.batch) * a.cache.heads;
-    if (a.cluster) return launch_cluster(k_kv4_step<C, BF16>, units, a.cluster, kStepThreads, C::SMEM, st, a);
-    k_kv4_step<C, BF16><<<a.runs, kStepThreads, C::SMEM, st>>>(a);
+    if (a.cluster) return launch_cluster(k_kv4_step<C, BF16>, units, a.cluster, C::THREADS, C::SMEM, st, a);
+    k_kv4_step<C, BF16><<<a.runs, C::THREADS, C::SMEM, st>>>(a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     constexpr int kJoinRows = 256 / D;  // rows of a CTA of k_kv4_join
@@ -260,6 +260,7 @@ template <int D, bool BF16>
 cudaError_t run_attention(const Kv4Attn& a, int nt, int sms, cudaStream_t st) {
     if (nt == 1) return run_step<D, 1, BF16>(a, st);
     if (nt == 2) return run_step<D, 2, BF16>(a, st);
+    if (nt == 3) return run_step<D, 3, BF16>(a, st);
     const cudaError_t e = run_step<D, 4, BF16>(a, st);
     return e == cudaSuccess && a.prompt_tiles ? run_prompt<D, BF16>(a, sms, st) : e;
 }

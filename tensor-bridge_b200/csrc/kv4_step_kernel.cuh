@@ -36,8 +36,8 @@
 // workspace for k_kv4_join.  Short sequences need no such plan: a cluster of
 // up to eight CTAs shares a unit and joins through distributed shared memory,
 // in one launch.  Within a CTA one warp looks pages up and issues
-// the bulk copies, a whole tile of 256 tokens by its 16 lanes at once, and
-// goes on into the next unit while eight warps compute, each on its own 32
+// the bulk copies, a whole tile of 256 or 384 tokens by its lanes at once, and
+// goes on into the next unit while the other warps compute, each on its own 32
 // tokens of a tile with its own o, m, l, merged once per unit in a fixed order.
 #pragma once
 
@@ -69,36 +69,41 @@ struct Kv4Attn {
 // Bit of the device error word: a sequence has more rows than max_rows.
 enum : int { kErrRows = 4 };
 
-constexpr int kStepWarps = 8;                        // that compute; one more loads
-constexpr int kStepThreads = 32 * (kStepWarps + 4);  // the loading warp's group of four: three of them idle
-constexpr int kStepChunk = 32;                       // tokens of a warp's share of a tile
-constexpr int kStepTile = kStepChunk * kStepWarps;
+constexpr int kStepChunk = 32;     // tokens of a warp's share of a tile
 // A row's maximum before it has seen a score: finite, so that differences are
 // ordinary numbers; every score passes it.
 constexpr float kNoMax = -1e38f;
 constexpr int kStepRowsMost = 32;  // packed rows of a (sequence, KV head)
 
+// NT tiles of eight rows.  Eight computing warps, and twelve for two tiles,
+// where one CTA is all that an SM holds and eight leave its pipes idle (16 rows,
+// 8 sequences of 10000 tokens, 8 KV heads of 128: 41.9 us with eight).
 template <int D_, int NT_>
 struct StepCfg {
     static constexpr int D = D_, NT = NT_;
+    static constexpr int WARPS = NT == 2 ? 12 : 8;        // that compute
+    static constexpr int THREADS = 32 * (WARPS + 4);      // the loading warp's group of four: three of them idle
+    static constexpr int TILE = kStepChunk * WARPS;       // tokens
+    static constexpr int GRAN_MOST = WARPS == 8 ? 8 : 7;  // log2 of a power of two that divides the tile
     static constexpr int ROWS = 8 * NT;
     static constexpr int TOKEN_BYTES = D / 2 + D / 16;  // of K or of V
-    static constexpr int STAGE = kStepTile * TOKEN_BYTES * 2;
+    static constexpr int STAGE = TILE * TOKEN_BYTES * 2;
     static constexpr int ST = D == 64 ? 3 : 2;
     static constexpr int OFF_MERGE = ST * STAGE;
-    static constexpr int OFF_Q = OFF_MERGE + kStepWarps * ROWS * (D + 4) * 4;
+    static constexpr int OFF_Q = OFF_MERGE + WARPS * ROWS * (D + 4) * 4;
     static constexpr int OFF_ML = OFF_Q + NT * (D / 16) * 32 * 8;
-    static constexpr int OFF_SCALE = OFF_ML + kStepWarps * ROWS * 2 * 4;
+    static constexpr int OFF_SCALE = OFF_ML + WARPS * ROWS * 2 * 4;
     static constexpr int OFF_INFO = OFF_SCALE + ROWS * 4;
-    static constexpr int OFF_BAR = OFF_INFO + ST * kStepWarps * 8;
+    static constexpr int OFF_BAR = OFF_INFO + ST * WARPS * 8;
     static constexpr int OFF_SUMS = OFF_BAR + 2 * ST * 8;
-    static constexpr int SMEM = OFF_SUMS + (kStepThreads / 32 + 3) * 8;
+    static constexpr int SMEM = OFF_SUMS + (THREADS / 32 + 3) * 8;
     // Registers a thread: at launch, then of the loading group and of the
     // computing warps.  The split never asks for more than the launch held.
     static constexpr int CTAS = NT == 1 ? 2 : 1;
-    static constexpr int REGS = CTAS == 2 ? 80 : 168, REGS_LOAD = CTAS == 2 ? 32 : 40,
-                         REGS_COMPUTE = CTAS == 2 ? 104 : 232;
-    static_assert(128 * REGS_LOAD + 32 * kStepWarps * REGS_COMPUTE <= kStepThreads * REGS, "registers of the launch");
+    static constexpr int REGS = NT == 1 ? 80 : NT == 2 ? 128 : 168;
+    static constexpr int REGS_LOAD = NT >= 3 ? 40 : 32, REGS_COMPUTE = NT == 1 ? 104 : NT == 2 ? 160 : 232;
+    static_assert(128 * REGS_LOAD + 32 * WARPS * REGS_COMPUTE <= THREADS * REGS, "registers of the launch");
+    static_assert(SMEM <= 227 * 1024 / CTAS - 1024 * (CTAS - 1), "shared memory");
     static constexpr int SLOT = ROWS * (D + 2);  // floats of a partial result: o [ROWS x D], m, l
 };
 
@@ -170,8 +175,10 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 
 // log2 of the tokens of a chunk, in which sequences are split: a page's, but 32
-// at least (a warp's share) and 256 at most (a tile).
-TB_KV4_HD int step_gran(int page_shift) { return page_shift < 5 ? 5 : page_shift > 8 ? 8 : page_shift; }
+// at least (a warp's share) and `most` at most (it divides a tile).
+TB_KV4_HD int step_gran(int page_shift, int most) {
+    return page_shift < 5 ? 5 : page_shift > most ? most : page_shift;
+}
 
 // Adds a partial result (u, li, mi) to (v, l, top).  A part that saw nothing
 // of the row has kNoMax, l = 0 and o = 0, or NaN, which stays.
@@ -195,10 +202,11 @@ struct StepSeq {
     __device__ __forceinline__ long long total(int heads) const { return static_cast<long long>(heads) * chunks; }
 };
 
+template <class C>
 __device__ __forceinline__ StepSeq step_seq(const Kv4Attn& a, int b) {
     StepSeq s;
     s.q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
-    s.span = kv4_span(s.q.pos0, s.q.pos0 + s.q.n - 1, s.q.len, a.window, a.sinks, step_gran(a.cache.page_shift));
+    s.span = kv4_span(s.q.pos0, s.q.pos0 + s.q.n - 1, s.q.len, a.window, a.sinks, step_gran(a.cache.page_shift, C::GRAN_MOST));
     const long long rows = static_cast<long long>(s.q.n) * a.group;
     s.chunks = rows > 0 && rows <= a.step_rows ? kv4_span_chunks(s.span) : 0;
     return s;
@@ -254,21 +262,21 @@ __device__ __forceinline__ void kv4_store_row(const Kv4Attn& a, int first, int r
 }
 
 template <class C, bool BF16>
-__global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Attn a) {
-    constexpr int D = C::D, NT = C::NT, ROWS = C::ROWS, ST = C::ST;
+__global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn a) {
+    constexpr int D = C::D, NT = C::NT, ROWS = C::ROWS, ST = C::ST, WARPS = C::WARPS;
     constexpr int KS = D / 16;   // k-steps of K Q^T
     constexpr int MT = D / 16;   // 16-row tiles of V^T
     extern __shared__ __align__(128) uint8_t smem[];
     float* merge = reinterpret_cast<float*>(smem + C::OFF_MERGE);
     uint2* qfrag = reinterpret_cast<uint2*>(smem + C::OFF_Q);
     float* sm_m = reinterpret_cast<float*>(smem + C::OFF_ML);
-    float* sm_l = sm_m + kStepWarps * ROWS;
+    float* sm_l = sm_m + WARPS * ROWS;
     float* sm_scale = reinterpret_cast<float*>(smem + C::OFF_SCALE);
     int2* info = reinterpret_cast<int2*>(smem + C::OFF_INFO);  // per stage and warp: first token, flags
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t* empty = full + ST;
     long long* sums = reinterpret_cast<long long*>(smem + C::OFF_SUMS);  // one per warp, then the result
-    volatile int* abort = reinterpret_cast<volatile int*>(sums + kStepThreads / 32 + 2);
+    volatile int* abort = reinterpret_cast<volatile int*>(sums + C::THREADS / 32 + 2);
 
     volatile int* failed = abort + 1;  // by a computing warp, before its second barrier of a unit
 
@@ -278,7 +286,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], kStepWarps);
+            mbar_init(&empty[i], WARPS);
         }
         fence_barrier_init();
         *abort = 0;
@@ -293,7 +301,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
     if (a.cluster) {
         const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
         b = unit / a.cache.heads;
-        const StepSeq s = step_seq(a, b);
+        const StepSeq s = step_seq<C>(a, b);
         if (tid == 0) step_report(a, s);
         if (s.chunks == 0) return;  // every CTA of the cluster
         const int from = static_cast<int>(run_start(s.chunks, a.cluster, rank));
@@ -302,10 +310,10 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
     } else {
         // The chunks of all sequences and of those before each one: a thread
         // takes the sequences tid, tid + 384, ...
-        constexpr int kWarps = kStepThreads / 32;
+        constexpr int kWarps = C::THREADS / 32;
         long long mine = 0, sum = 0;
-        for (int i = tid; i < a.rows.batch; i += kStepThreads) {
-            const StepSeq s = step_seq(a, i);
+        for (int i = tid; i < a.rows.batch; i += C::THREADS) {
+            const StepSeq s = step_seq<C>(a, i);
             if (my_run == 0) step_report(a, s);
             const long long w = s.total(a.cache.heads);
             if (i == tid) mine = w;
@@ -318,9 +326,9 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
         left = run_start(total, runs, my_run + 1) - from;
         if (left <= 0) return;
         long long before = 0;
-        for (int b0 = 0; b0 < a.rows.batch && before <= from; b0 += kStepThreads) {
+        for (int b0 = 0; b0 < a.rows.batch && before <= from; b0 += C::THREADS) {
             const int i = b0 + tid;
-            const long long w = b0 == 0 ? mine : i < a.rows.batch ? step_seq(a, i).total(a.cache.heads) : 0;
+            const long long w = b0 == 0 ? mine : i < a.rows.batch ? step_seq<C>(a, i).total(a.cache.heads) : 0;
             long long upto = w;  // inclusive sum over the CTA's threads
             for (int d = 1; d < 32; d <<= 1) {
                 const long long o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
@@ -346,12 +354,12 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
         off = sums[kWarps + 1];
     }
 
-    // Chunk geometry.  A stage holds a tile of 256 tokens as whole chunks; a
-    // chunk is a page's block of this head as it lies in the cache, two of
-    // them for 16-token pages, or 256 tokens of a larger page.
-    const int shift = a.cache.page_shift, gs = step_gran(shift);
+    // Chunk geometry.  A stage holds a tile of tokens as whole chunks; a chunk
+    // is a page's block of this head as it lies in the cache, two of them for
+    // 16-token pages, or some tokens of a larger page.
+    const int shift = a.cache.page_shift, gs = step_gran(shift, C::GRAN_MOST);
     const uint32_t gran = 1u << gs;
-    const int per_tile = kStepTile >> gs;
+    const int per_tile = C::TILE >> gs;
     const uint32_t codes = kv4_codes_bytes(a.cache), scales = kv4_scales_bytes(a.cache);
     const uint32_t block_tokens = shift == 4 ? 16u : gran;  // contiguous in the stage: Kc, Ks, Vc, Vs
     const uint32_t at_ks = block_tokens * (D / 2), at_vc = at_ks + block_tokens * (D / 16),
@@ -359,16 +367,16 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
 
     int stage = 0;
     uint32_t phase = 0;
-    if (warp >= kStepWarps) {
+    if (warp >= WARPS) {
         reg_dec<C::REGS_LOAD>();
-        if (warp > kStepWarps) return;
-        // ---- the loading warp: lane i < 16 looks after tokens 16 i .. + 15 of a tile ----
+        if (warp > WARPS) return;
+        // ---- the loading warp: lane i looks after tokens 16 i .. + 15 of a tile ----
         const int sub = lane * 16;                       // place in the tile
         const int entry = sub >> gs;                     // its chunk of the tile
-        const bool leads = lane < 16 && (sub & static_cast<int>(block_tokens - 1)) == 0;  // first of a block
+        const bool leads = lane < 2 * WARPS && (sub & static_cast<int>(block_tokens - 1)) == 0;  // first of a block
         uint32_t filled = 0;
         while (left > 0 && b < a.rows.batch) {
-            const StepSeq s = step_seq(a, b);
+            const StepSeq s = step_seq<C>(a, b);
             if (off >= s.total(a.cache.heads)) {
                 off -= s.total(a.cache.heads);
                 ++b;
@@ -391,7 +399,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
             auto look = [&](int q, int& tok, int& page) {
                 tok = -1;
                 page = -1;
-                if (lane < 16 && q + entry < c1) {
+                if (lane < 2 * WARPS && q + entry < c1) {
                     tok = (kv4_span_chunk(s.span, q + entry) << gs) + (sub & static_cast<int>(gran - 1));
                     if (tok < s.q.len) page = table[tok >> shift];
                 }
@@ -405,21 +413,21 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
                 if (inside && !ok) atomicOr(&g_tb_device_error, kErrPage);
                 const uint32_t have = __ballot_sync(0xFFFFFFFFu, ok);
                 const uint32_t copies = __ballot_sync(0xFFFFFFFFu, ok && leads);
-                if (lane < 16 && (lane & 1) == 0) {
+                if (lane < 2 * WARPS && (lane & 1) == 0) {
                     const uint32_t two = (have >> lane) & 3u;
                     const bool open = two == 3u && tok + kStepChunk <= open_end &&
                                       (tok >= open_low || tok + kStepChunk <= a.sinks);
-                    info[stage * kStepWarps + lane / 2] = make_int2(tok, static_cast<int>(two | (open ? 4u : 0u)));
+                    info[stage * WARPS + lane / 2] = make_int2(tok, static_cast<int>(two | (open ? 4u : 0u)));
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(&full[stage], __popc(copies) * block_bytes);
                 __syncwarp();
                 uint8_t* dst = smem + stage * C::STAGE + (sub / static_cast<int>(block_tokens)) * block_bytes;
-                if (shift <= 8) {
+                if (shift <= gs) {
                     if (ok && leads)
                         bulk_load(dst, blocks + static_cast<unsigned long long>(static_cast<uint32_t>(page)) * a.cache.page_stride,
                                   block_bytes, &full[stage]);
-                } else if (ok && leads) {  // lane 0: a tile of a larger page, part by part
+                } else if (ok && leads) {  // a chunk of a larger page, part by part
                     const uint32_t place = static_cast<uint32_t>(tok) & ((1u << shift) - 1u);
                     const uint8_t* src =
                         blocks + static_cast<unsigned long long>(static_cast<uint32_t>(page)) * a.cache.page_stride;
@@ -462,7 +470,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
 
     // A CTA of a cluster has one pass, with or without chunks.
     for (bool once = a.cluster != 0; (once || left > 0) && b < a.rows.batch; once = false) {
-        const StepSeq s = step_seq(a, b);
+        const StepSeq s = step_seq<C>(a, b);
         if (off >= s.total(a.cache.heads) && left > 0) {
             off -= s.total(a.cache.heads);
             ++b;
@@ -478,7 +486,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
         // Queries in fragment order: lane (g, c) of k-step ks holds, for row
         // g, the values d = (D/4) c + 4 ks .. + 3, each pair swapped as the
         // converter leaves a byte's two codes.
-        for (int r = warp; r < ROWS; r += kStepWarps) {
+        for (int r = warp; r < ROWS; r += WARPS) {
             uint2 v = make_uint2(0u, 0u);
             // The factor is taken positive, its sign into q: the largest product
             // is the largest score.  Not zero, which would make NaN of -inf.
@@ -511,7 +519,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
             }
             if (lane == 0) sm_scale[r] = scale;
         }
-        named_bar_sync(1, 32 * kStepWarps);
+        named_bar_sync(1, 32 * WARPS);
 
         float sf[NT][2];  // score -> log2 units, of rows 8 nt + 2c, + 1
         float m[NT][2], l[NT][2];
@@ -536,7 +544,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
                 *failed = 1;
                 break;
             }
-            const int2 what = info[stage * kStepWarps + warp];
+            const int2 what = info[stage * WARPS + warp];
             const int tok0 = what.x;
             const uint32_t have = what.y & 3u;
             const bool open = what.y & 4;
@@ -610,7 +618,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
                 }
             }
 
-            if (!open) {
+            if (__builtin_expect(!open, 0)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -634,7 +642,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
                 for (int e = 0; e < 2; ++e)
                     past |= fmaf(fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2])),
                                  sf[nt][e], -m[nt][e]) > 8.0f;
-            if (__any_sync(0xFFFFFFFFu, past)) {
+            if (__builtin_expect(__any_sync(0xFFFFFFFFu, past), 0)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -684,7 +692,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
                     asm volatile("ld.shared.u8 %0, [%1];"
                                  : "=r"(sv[k]) : "r"(sb + ((k & 1) * v_pair + (k >> 1) * 8) * (D / 16)));
                 }
-                if (!open) {
+                if (__builtin_expect(!open, 0)) {
                     // A token that a row does not see adds nothing to it, NaN
                     // or not: 0 * NaN is avoided by zeroing the scale, and a
                     // NaN block is put into the rows that do see its token.
@@ -755,7 +763,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
                     sm_l[warp * ROWS + 8 * nt + 2 * c + e] = l[nt][e];
                 }
             }
-        named_bar_sync(1, 32 * kStepWarps);
+        named_bar_sync(1, 32 * WARPS);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -763,7 +771,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
                 const int r = 8 * nt + 2 * c + e;
                 float top = kNoMax;
 #pragma unroll
-                for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sm_m[w * ROWS + r]);
+                for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_m[w * ROWS + r]);
                 const float f = ex2(m[nt][e] - top);
                 float* at = merge + (warp * ROWS + r) * (D + 4) + g * (D / 8);
 #pragma unroll
@@ -773,19 +781,19 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
                                     o[2 * k + 1][nt][e + 2] * f);
                 }
             }
-        named_bar_sync(1, 32 * kStepWarps);
+        named_bar_sync(1, 32 * WARPS);
         if (*failed && a.cluster == 0) return;  // all of them
         const bool partial = !(c0 == 0 && c1 == s.chunks) && a.cluster == 0;
         float* slot = partial ? step_slot<C>(a.ws, my_run, c0 == 0 ? 1 : 0) : nullptr;
-        for (int x = tid; x < row_count * (D / 4); x += kStepWarps * 32) {
+        for (int x = tid; x < row_count * (D / 4); x += WARPS * 32) {
             const int r = x / (D / 4), d = 4 * (x % (D / 4));
             float top = kNoMax;
 #pragma unroll
-            for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, sm_m[w * ROWS + r]);
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_m[w * ROWS + r]);
             float sum = 0.0f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kStepWarps; ++w) {
+            for (int w = 0; w < WARPS; ++w) {
                 sum += sm_l[w * ROWS + r] * ex2(sm_m[w * ROWS + r] - top);
                 const float4 u = *reinterpret_cast<const float4*>(merge + (w * ROWS + r) * (D + 4) + d);
                 v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
@@ -810,7 +818,7 @@ __global__ void __launch_bounds__(kStepThreads, C::CTAS) k_kv4_step(const Kv4Att
             __syncwarp();
             cluster_sync();
             const int rank = static_cast<int>(cluster_ctarank());
-            for (int x = tid * a.cluster + rank; x < row_count * (D / 4); x += 32 * kStepWarps * a.cluster) {
+            for (int x = tid * a.cluster + rank; x < row_count * (D / 4); x += 32 * WARPS * a.cluster) {
                 const int r = x / (D / 4), d = 4 * (x % (D / 4));
                 float top = kNoMax, l = 0.0f;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -838,12 +846,12 @@ __global__ void __launch_bounds__(256) k_kv4_join(const Kv4Attn a) {
     __shared__ float4 part_v[4][256 / 4];
     __shared__ float2 part_ml[4][256 / 4];
     const int b = blockIdx.x / a.cache.heads, head = blockIdx.x - b * a.cache.heads;
-    const StepSeq s = step_seq(a, b);
+    const StepSeq s = step_seq<C>(a, b);
     const int row0 = blockIdx.y * (64 / LANES);
     if (s.chunks == 0 || row0 >= s.q.n * a.group) return;
     long long sum = 0, sum_before = 0;
     for (int i = threadIdx.x; i < a.rows.batch; i += blockDim.x) {
-        const long long w = step_seq(a, i).total(a.cache.heads);
+        const long long w = step_seq<C>(a, i).total(a.cache.heads);
         sum += w;
         if (i < b) sum_before += w;
     }
