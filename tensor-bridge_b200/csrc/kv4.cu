@@ -129,8 +129,8 @@ dim3 copy_grid(const Kv4Copy& a, int per_cta, unsigned y) {
 template <bool BF16>
 cudaError_t run_append(const Kv4Copy& a, cudaStream_t st, int sms) {
     unsigned y;
-    if (many_rows(a, 4, sms, &y)) k_kv4_append<BF16, 16><<<copy_grid(a, 16, y), kKv4CopyThreads, 0, st>>>(a);
-    else k_kv4_append<BF16, 4><<<copy_grid(a, 4, y), kKv4CopyThreads, 0, st>>>(a);
+    if (many_rows(a, 4, sms, &y)) k_kv4_append<BF16, 32, 2><<<copy_grid(a, 32, y), kKv4CopyThreads, 0, st>>>(a);
+    else k_kv4_append<BF16, 4, 1><<<copy_grid(a, 4, y), kKv4CopyThreads, 0, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -295,6 +295,10 @@ tb_status tb_kv4_append(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_f
     int sms = 0;
     const tb_status s = check_copy(cache, rows, fmt, k, k_stride, v, v_stride, &a, &sms);
     if (s != TB_OK || a.rows.batch == 0 || a.rows.rows == 0) return s;
+    a.rk = 1.0f / a.cache.k_scale;
+    a.rv = 1.0f / a.cache.v_scale;
+    a.r6k = 1.0f / (6.0f * a.cache.k_scale);
+    a.r6v = 1.0f / (6.0f * a.cache.v_scale);
     a.lanes_per_row = static_cast<uint32_t>(a.cache.dim) / 16;
     a.magic = (65536u + a.lanes_per_row - 1) / a.lanes_per_row;
     return launched(fmt == TB_FMT_BF16 ? run_append<true>(a, stream, sms) : run_append<false>(a, stream, sms));

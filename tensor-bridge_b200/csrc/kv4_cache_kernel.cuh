@@ -38,6 +38,7 @@ struct Kv4Copy {
     long long k_stride, v_stride;  // elements from one row to the next
     uint32_t lanes_per_row;        // items of a (row, head)
     uint32_t magic;                // ceil(65536 / lanes_per_row)
+    float rk, rv, r6k, r6v;        // append: 1 / g and 1 / (6 g) of K and V
 };
 
 constexpr int kKv4CopyThreads = 256;
@@ -88,66 +89,65 @@ __device__ __forceinline__ float e4m3_value(uint32_t byte) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(cvt_e4m3x2(static_cast<uint16_t>(byte)))));
 }
 
-// Scale byte of a block whose largest magnitude is `amax` (not NaN).  The
-// borders between two E4M3 values lie at 6 g times their mean, m; 6 m has at
-// most 7 significant bits, so `__fmul_rd(6 m, g)` is the exact border rounded
-// down to FP32, and the FP32 number amax exceeds the border exactly when it
-// exceeds that.  The division only finds the value below: where its rounding
-// picks a neighbour, the border compared against still decides.
-__device__ __forceinline__ uint32_t kv4_scale_byte(float amax, float g) {
-    const float q = fminf(amax / (6.0f * g), 448.0f);
+// Scale byte of a block whose largest magnitude is `amax` (not NaN); r6g is
+// 1 / (6 g).  The borders between two E4M3 values lie at 6 g times their mean,
+// m; 6 m has at most 7 significant bits, so `__fmul_rd(6 m, g)` is the exact
+// border rounded down to FP32, and the FP32 number amax exceeds the border
+// exactly when it exceeds that.  The product with r6g only finds the value
+// below: where its rounding picks a neighbour, the border compared against
+// still decides.
+__device__ __forceinline__ uint32_t kv4_scale_byte(float amax, float g, float r6g) {
+    const float q = fminf(amax * r6g, 448.0f);
     // largest E4M3 value not above q
     uint32_t c;
     if (q < 0.015625f) c = static_cast<uint32_t>(q * 512.0f);  // subnormal: multiples of 2^-9
     else c = (__float_as_uint(q) >> 20) - (120u << 3);         // exponent bias 127 -> 7, three mantissa bits
     if (c >= 126u) return 126u;
-    const float mid = 0.5f * (e4m3_value(c) + e4m3_value(c + 1));
-    return amax > __fmul_rd(6.0f * mid, g) ? c + 1 : c;
+    const uint32_t two = cvt_e4m3x2(static_cast<uint16_t>(c * 0x101u + 0x100u));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&two));
+    return amax > __fmul_rd(3.0f * (v.x + v.y), g) ? c + 1 : c;
 }
 
-// Codes of 16 values for the scale value s > 0: eight bytes, first value in
-// the high nibble.  The border above magnitude i lies at t_i s g with t_i s
-// exact in FP32, so x passes it exactly when |x| > __fmul_rd(t_i s, g).  The
-// converter rounds y = |x| / (s g) to the nearest E2M1 value; y is off by at
-// most 2^-22 of itself (two roundings of the reciprocal's product and one
-// here), so where both ends of that interval convert alike no border lies
-// between and the code is right; else the borders are compared.
-__device__ __forceinline__ void kv4_codes(const float (&x)[16], float s, float g, uint32_t (&out)[2]) {
-    const float inv = 1.0f / (s * g);
-    const bool plain = inv < 1e30f && s * g < 1e30f && s * g > 1e-30f;  // the interval's ends are ordinary numbers
+// Eight values to codes by the converter, first value in the high nibble of
+// the first byte.
+__device__ __forceinline__ uint32_t cvt_e2m1_x8(const float (&x)[8], float by) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %1, %2;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %3, %4;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %5, %6;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %7, %8;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(r)
+        : "f"(x[0] * by), "f"(x[1] * by), "f"(x[2] * by), "f"(x[3] * by), "f"(x[4] * by), "f"(x[5] * by),
+          "f"(x[6] * by), "f"(x[7] * by));
+    return r;
+}
+
+// Codes of eight values for the scale value s > 0; rg is 1 / g.  The border
+// above magnitude i lies at t_i s g with t_i s exact in FP32, so x passes it
+// exactly when |x| > __fmul_rd(t_i s, g).  The converter rounds x / (s g) to
+// the nearest E2M1 value; here that quotient is off by less than 2^-21 of
+// itself (the reciprocal of s 2^-23, three products and rg 2^-24 each), so
+// where it converts alike 2^-20 below and above no border lies between and the
+// code is right; else the borders are compared.
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], float s, float g, float rg) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    inv *= rg;
+    const uint32_t lo = cvt_e2m1_x8(x, inv * (1.0f - 0x1p-20f)), hi = cvt_e2m1_x8(x, inv * (1.0f + 0x1p-20f));
+    if (lo == hi) return lo;
+    uint32_t word = 0;
+#pragma unroll 1
+    for (int i = 0; i < 7; ++i) {
+        const float mids[7] = {0.25f, 0.75f, 1.25f, 1.75f, 2.5f, 3.5f, 5.0f};
+        const float border = __fmul_rd(mids[i] * s, g);
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        uint32_t word = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x0 = x[8 * w + 2 * j], x1 = x[8 * w + 2 * j + 1];
-            const float y0 = x0 * inv, y1 = x1 * inv;
-            constexpr float kLess = 1.0f - 0x1p-20f, kMore = 1.0f + 0x1p-20f;
-            uint32_t lo, hi;
-            asm("{\n\t.reg .b8 b;\n\t.reg .b16 h;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u16.u8 h, b;\n\tcvt.u32.u16 %0, h;\n\t}"
-                : "=r"(lo)
-                : "f"(y0 * kLess), "f"(y1 * kLess));
-            asm("{\n\t.reg .b8 b;\n\t.reg .b16 h;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\tcvt.u16.u8 h, b;\n\tcvt.u32.u16 %0, h;\n\t}"
-                : "=r"(hi)
-                : "f"(y0 * kMore), "f"(y1 * kMore));
-            if (lo != hi || !plain) {
-                const float mids[7] = {0.25f, 0.75f, 1.25f, 1.75f, 2.5f, 3.5f, 5.0f};
-                uint32_t m0 = 0, m1 = 0;
-                for (int i = 0; i < 7; ++i) {
-                    const float border = __fmul_rd(mids[i] * s, g);
-                    m0 += fabsf(x0) > border;
-                    m1 += fabsf(x1) > border;
-                }
-                m0 |= (__float_as_uint(x0) >> 28) & 8u;
-                m1 |= (__float_as_uint(x1) >> 28) & 8u;
-                lo = (m0 << 4) | m1;
-            }
-            word |= lo << (8 * j);
-        }
-        out[w] = word;
+        for (int j = 0; j < 8; ++j) word += static_cast<uint32_t>(fabsf(x[j]) > border) << (8 * (j / 2) + (j & 1 ? 0 : 4));
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) word |= ((__float_as_uint(x[j]) >> 31) << 3) << (8 * (j / 2) + (j & 1 ? 0 : 4));
+    return word;
 }
 
 template <bool BF16>
@@ -166,8 +166,9 @@ __device__ __forceinline__ void unpack8(const uint4& u, float* x) {
     }
 }
 
-// One lane quantises one block of 16 values.
-template <bool BF16, int ROWS>
+// One lane quantises one block of 16 values; the values of UNROLL blocks are on
+// their way before the first is worked on.
+template <bool BF16, int ROWS, int UNROLL>
 __global__ void __launch_bounds__(kKv4CopyThreads) k_kv4_append(const Kv4Copy a) {
     __shared__ Kv4Places<ROWS> s;
     const int row0 = blockIdx.x * ROWS;
@@ -178,34 +179,56 @@ __global__ void __launch_bounds__(kKv4CopyThreads) k_kv4_append(const Kv4Copy a)
     for (int pair = blockIdx.y * warps + threadIdx.x / 32; pair < 2 * a.cache.heads; pair += gridDim.y * warps) {
         const bool is_v = pair >= a.cache.heads;
         const int head = is_v ? pair - a.cache.heads : pair;
-        const float g = is_v ? a.cache.v_scale : a.cache.k_scale;
+        const float g = is_v ? a.cache.v_scale : a.cache.k_scale, rg = is_v ? a.rv : a.rk, r6g = is_v ? a.r6v : a.r6k;
         const uint16_t* src = static_cast<const uint16_t*>(is_v ? a.v : a.k) + static_cast<size_t>(head) * a.cache.dim;
         const long long stride = is_v ? a.v_stride : a.k_stride;
         uint8_t* block = a.cache.data + static_cast<size_t>(head) * kv4_head_bytes(a.cache) +
                          (is_v ? codes + scales : 0u);
-        for (uint32_t t = threadIdx.x & 31; t < items; t += 32) {
-            const uint32_t r = (t * a.magic) >> 16, i = t - r * a.lanes_per_row;
-            const unsigned long long page = s.page[r];
-            if (page == ~0ull) continue;
-            const uint4* p = reinterpret_cast<const uint4*>(src + static_cast<long long>(row0 + r) * stride + 16 * i);
-            const uint4 u0 = p[0], u1 = p[1];
-            float x[16];
-            unpack8<BF16>(u0, x);
-            unpack8<BF16>(u1, x + 8);
-            float amax = 0.0f;
-            bool nan = false;
+        for (uint32_t t0 = threadIdx.x & 31; t0 < items; t0 += 32 * UNROLL) {
+            uint4 u[UNROLL][2];
+            bool on[UNROLL];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                amax = fmaxf(amax, fabsf(x[j]));
-                nan |= x[j] != x[j];
+            for (int k = 0; k < UNROLL; ++k) {
+                const uint32_t t = t0 + 32 * k;
+                const uint32_t r = (t * a.magic) >> 16, i = t - r * a.lanes_per_row;
+                on[k] = t < items && s.page[t < items ? r : 0] != ~0ull;
+                if (on[k]) {
+                    const uint4* p = reinterpret_cast<const uint4*>(src + static_cast<long long>(row0 + r) * stride + 16 * i);
+                    u[k][0] = p[0];
+                    u[k][1] = p[1];
+                }
             }
-            const uint32_t sb = nan ? 0x7Fu : kv4_scale_byte(amax, g);
-            uint32_t w[2] = {0u, 0u};
-            if (sb != 0u && !nan) kv4_codes(x, e4m3_value(sb), g, w);
-            uint8_t* at = block + page;
-            const uint32_t tok = static_cast<uint32_t>(s.place[r]);
-            *reinterpret_cast<uint2*>(at + tok * (a.cache.dim / 2) + 8 * i) = make_uint2(w[0], w[1]);
-            at[codes + tok * (a.cache.dim / 16) + i] = static_cast<uint8_t>(sb);
+#pragma unroll
+            for (int k = 0; k < UNROLL; ++k) {
+                if (!on[k]) continue;
+                const uint32_t t = t0 + 32 * k;
+                const uint32_t r = (t * a.magic) >> 16, i = t - r * a.lanes_per_row;
+                // The largest magnitude: without their signs the values order
+                // like their bits, NaN above all.
+                constexpr uint32_t kAbs = 0x7FFF7FFFu;
+                uint32_t m = __vmaxu2(__vmaxu2(__vmaxu2(u[k][0].x & kAbs, u[k][0].y & kAbs),
+                                               __vmaxu2(u[k][0].z & kAbs, u[k][0].w & kAbs)),
+                                      __vmaxu2(__vmaxu2(u[k][1].x & kAbs, u[k][1].y & kAbs),
+                                               __vmaxu2(u[k][1].z & kAbs, u[k][1].w & kAbs)));
+                m = max(m & 0xFFFFu, m >> 16);
+                const bool nan = m > (BF16 ? 0x7F80u : 0x7C00u);
+                const float amax = BF16 ? __uint_as_float(m << 16)
+                                        : __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
+                const uint32_t sb = nan ? 0x7Fu : kv4_scale_byte(amax, g, r6g);
+                uint2 w = make_uint2(0u, 0u);
+                if (sb != 0u && !nan) {
+                    const float sv = e4m3_value(sb);
+                    float x[8];
+                    unpack8<BF16>(u[k][0], x);
+                    w.x = kv4_codes(x, sv, g, rg);
+                    unpack8<BF16>(u[k][1], x);
+                    w.y = kv4_codes(x, sv, g, rg);
+                }
+                uint8_t* at = block + s.page[r];
+                const uint32_t tok = static_cast<uint32_t>(s.place[r]);
+                *reinterpret_cast<uint2*>(at + tok * (a.cache.dim / 2) + 8 * i) = w;
+                at[codes + tok * (a.cache.dim / 16) + i] = static_cast<uint8_t>(sb);
+            }
         }
     }
 }
@@ -213,7 +236,7 @@ __global__ void __launch_bounds__(kKv4CopyThreads) k_kv4_append(const Kv4Copy a)
 // One lane reads back eight values; UNROLL of them are loaded before the first
 // is stored, to keep enough of the memory's latency in flight.
 template <bool BF16, int ROWS, int UNROLL>
-__global__ void __launch_bounds__(kKv4CopyThreads) k_kv4_read(const Kv4Copy a) {
+__global__ void __launch_bounds__(kKv4CopyThreads, 4) k_kv4_read(const Kv4Copy a) {
     __shared__ Kv4Places<ROWS> s;
     const int row0 = blockIdx.x * ROWS;
     kv4_find_rows<ROWS>(a, row0, s);
