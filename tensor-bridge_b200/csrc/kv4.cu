@@ -154,27 +154,38 @@ struct AttnPlan {
     size_t bytes;       // of both kernels' partial results
 };
 
-AttnPlan plan_attention(int batch, int heads, int dim, int page_shift, int group, int max_rows, int max_len, int sms) {
+AttnPlan plan_attention(int batch, int heads, int dim, int page_shift, int group, int max_rows, int max_len, int window,
+                        int sinks, int sms) {
     AttnPlan p{};
     const long long rows = static_cast<long long>(max_rows) * group;
+    // Tokens that a sequence's rows see at most.  A window can only lower it,
+    // and with it the bytes: tb_kv4_attention_workspace, which is told of none,
+    // asks for enough.
+    if (window > 0)
+        max_len = static_cast<int>(std::min<long long>(max_len, static_cast<long long>(window) + sinks + max_rows));
     p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
     p.runs = sms * (p.nt == 1 ? 2 : 1);
     // Clusters where they all fit on the GPU at once, a tile of tokens or more
-    // to a CTA; 8 rows, 8 KV heads of 128, pages of 16, one sequence of 1000,
-    // 4096, 16384 tokens: 7.2, 8.5, 17.3 us against 9.7, 10.4, 17.1 us in runs.
-    p.cluster = std::max(1, std::min(8, (max_len + 255) / 256));
-    if (max_len > 16384 || static_cast<long long>(batch) * heads * p.cluster > p.runs) p.cluster = 0;
+    // to a CTA and not many (a cluster waits for its longest sequence, runs of
+    // chunks share it): up to 1024 tokens, or 2560 where the clusters fill most
+    // of the GPU.  One row, 8 KV heads of 128, clusters against runs: 1 sequence
+    // of 1000 tokens 7.4, 10.6 us; 1 of 16384 17.3, 15.3 us; 4 of 16384 24.5,
+    // 28.5 us; 32 of 2000 23.5, 28.3 us; 1 of 32768 28.3, 19.7 us.
+    const long long units = static_cast<long long>(batch) * heads, room = p.runs / std::max(1ll, units);
+    const long long share = std::min(std::min(8ll, room), std::max(1ll, (max_len + 255ll) / 256));
+    if (share > 0 && max_len <= share * (units * share * 4 >= p.runs * 3ll ? 2560 : 1024))
+        p.cluster = static_cast<int>(share);
     p.min_run = std::max(1, 512 >> step_gran(page_shift, p.nt == 2 ? 7 : 8));
-    p.step_bytes = p.cluster ? 0 : static_cast<size_t>(p.runs) * 2 * (8 * p.nt) * (dim + 2) * sizeof(float);
+    p.step_bytes = p.cluster ? 0 : static_cast<size_t>(p.runs) * (sizeof(StepLink) + 2 * (8 * p.nt) * (dim + 2) * sizeof(float));
     p.splits = 1;
     p.bytes = p.step_bytes;
     if (rows > kStepRowsMost) {
         p.prompt_tiles = static_cast<int>((rows + kPromptRows - 1) / kPromptRows);
         // Fewer units than SMs: a unit's tokens are shared, 512 at least to each.
-        const long long units = static_cast<long long>(batch) * heads * p.prompt_tiles;
-        p.splits = static_cast<int>(std::max(1ll, std::min(sms / std::max(units, 1ll), max_len / 512ll)));
+        const long long items = units * p.prompt_tiles;
+        p.splits = static_cast<int>(std::max(1ll, std::min(sms / std::max(items, 1ll), max_len / 512ll)));
         if (p.splits > 1)
-            p.bytes += static_cast<size_t>(units) * p.splits * kPromptRows * (dim + 2) * sizeof(float);
+            p.bytes += static_cast<size_t>(items) * p.splits * kPromptRows * (dim + 2) * sizeof(float);
     }
     return p;
 }
@@ -240,7 +251,7 @@ cudaError_t run_step(const Kv4Attn& a, cudaStream_t st) {
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     constexpr int kJoinRows = 256 / D;  // rows of a CTA of k_kv4_join
-    return launch_early(k_kv4_join<C, BF16>, dim3(units, (C::ROWS + kJoinRows - 1) / kJoinRows), 256, 0, st, a);
+    return launch_early(k_kv4_join<C, BF16>, dim3(a.runs, (C::ROWS + kJoinRows - 1) / kJoinRows), 256, 0, st, a);
 }
 
 template <int D, bool BF16>
@@ -252,7 +263,7 @@ cudaError_t run_prompt(const Kv4Attn& a, int sms, cudaStream_t st) {
     const int ctas = std::min(a.prompt_units * a.prompt_splits, sms);
     e = launch_early(k_kv4_prompt<C, BF16>, dim3(ctas), kPromptThreads, C::SMEM, st, a);
     if (e != cudaSuccess || a.prompt_splits == 1) return e;
-    k_kv4_prompt_join<C, BF16><<<dim3(a.prompt_units, kPromptRows / 32), 256, 0, st>>>(a);
+    k_kv4_prompt_join<C, BF16><<<dim3(a.prompt_units, kPromptRows * D / 256), 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -321,7 +332,7 @@ size_t tb_kv4_attention_workspace(const tb_kv4_cache* cache, const tb_kv4_rows* 
     Kv4Rows r{};
     if (check_cache(cache, &c) != TB_OK || check_rows(rows, c.page_shift, &r) != TB_OK) return 0;
     if (check_heads(cache, q_heads, max_rows, max_len) != TB_OK) return 0;
-    return plan_attention(r.batch, c.heads, c.dim, c.page_shift, q_heads / c.heads, std::min(max_rows, r.rows), max_len,
+    return plan_attention(r.batch, c.heads, c.dim, c.page_shift, q_heads / c.heads, std::min(max_rows, r.rows), max_len, 0, 0,
                           device_info(current_device()).sms)
         .bytes;
 }
@@ -361,7 +372,7 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     s = check_gpu(&sms);
     if (s != TB_OK) return s;
     const AttnPlan p = plan_attention(a.rows.batch, a.cache.heads, a.cache.dim, a.cache.page_shift, a.group,
-                                      std::min(max_rows, a.rows.rows), max_len, sms);
+                                      std::min(max_rows, a.rows.rows), max_len, window, sinks, sms);
     if (p.bytes) {
         if (!workspace || workspace_bytes < p.bytes) return refuse(TB_ERR_WORKSPACE, "workspace missing or too small");
         if (!aligned16(workspace)) return refuse(TB_ERR_ALIGNMENT, "workspace must be 16-byte aligned");

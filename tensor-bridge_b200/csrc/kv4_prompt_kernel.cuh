@@ -857,28 +857,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
 }
 
 // Joins the splits of the prompt kernel's units, in their order.  blockIdx.y
-// takes 32 of a unit's rows.
+// takes 256 / D of a unit's rows.
 template <class C, bool BF16>
 __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4Attn a) {
-    constexpr int D = C::D;
+    constexpr int D = C::D, LANES = D / 4;
     const PromptUnit u = prompt_unit(a, blockIdx.x * a.prompt_splits);
-    if (!u.any) return;
-    const int tiles = kv4_span_chunks(u.span);
-    const int r0 = blockIdx.y * 32, r1 = min(r0 + 32, u.row_count);
-    for (int x = r0 * (D / 4) + threadIdx.x; x < r1 * (D / 4); x += blockDim.x) {
-        const int r = x / (D / 4), d = 4 * (x % (D / 4));
-        float top = kNoMax, l = 0.0f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < a.prompt_splits; ++s) {
-            if (static_cast<long long>(tiles) * s / a.prompt_splits ==
-                static_cast<long long>(tiles) * (s + 1) / a.prompt_splits)
-                continue;  // no tiles, no result
+    const int quarter = threadIdx.x / 64, item = threadIdx.x % 64;
+    const int r = blockIdx.y * (64 / LANES) + item / LANES, d = 4 * (item % LANES);
+    if (!u.any || static_cast<int>(blockIdx.y) * (64 / LANES) >= u.row_count) return;
+    const bool valid = r < u.row_count;
+    const long long tiles = kv4_span_chunks(u.span);
+    float top = kNoMax, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (valid) {
+#pragma unroll 4
+        for (int s = quarter; s < a.prompt_splits; s += 4) {
+            if (tiles * s / a.prompt_splits == tiles * (s + 1) / a.prompt_splits) continue;  // no tiles, no result
             const float* slot = a.prompt_ws + (static_cast<size_t>(blockIdx.x) * a.prompt_splits + s) * C::SLOT_FLOATS;
             kv4_merge(top, l, v, slot[kPromptRows * D + r], slot[kPromptRows * (D + 1) + r],
                       *reinterpret_cast<const float4*>(slot + r * D + d));
         }
-        kv4_store_row<BF16, D>(a, u.q.first, u.row_base + r, u.head, d, v, top, l);
     }
+    join_and_store<BF16, D>(a, valid, u.q.first, u.row_base + r, u.head, d, top, l, v);
 }
 
 }  // namespace tb

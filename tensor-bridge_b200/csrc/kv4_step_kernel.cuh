@@ -108,10 +108,20 @@ struct StepCfg {
 };
 
 // A partial result belongs to CTA `run`: slot 0 for the unit that began in an
-// earlier CTA's run, slot 1 for one that begins here and goes on.
+// earlier CTA's run, slot 1 for one that begins here and goes on.  The slots
+// follow a StepLink of each run.
 template <class C>
-__device__ __forceinline__ float* step_slot(float* ws, int run, int slot) {
-    return ws + (static_cast<size_t>(run) * 2 + slot) * C::SLOT;
+__device__ __forceinline__ float* step_slot(const Kv4Attn& a, int run, int slot) {
+    return a.ws + static_cast<size_t>(a.runs) * 4 + (static_cast<size_t>(run) * 2 + slot) * C::SLOT;
+}
+
+// What a run leaves for k_kv4_join: the last run of the unit that begins in it
+// and goes on (-1: none does), and where the unit's rows belong.
+struct alignas(16) StepLink {
+    int last, first, rows, head;
+};
+__device__ __forceinline__ StepLink* step_link(const Kv4Attn& a, int run) {
+    return reinterpret_cast<StepLink*>(a.ws) + run;
 }
 
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -297,6 +307,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
     // This CTA's run of chunks: sequence b, offset `off` in it, `left` chunks.
     int b = 0;
     long long off = 0, left = 0;
+    long long end = 0, all_chunks = 0;  // of this run in all chunks laid end to end; their number
+    int all_runs = 0;
     const int my_run = blockIdx.x;
     if (a.cluster) {
         const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
@@ -321,10 +333,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
         }
         const long long total = block_sum(sum, sums);
         const int runs = step_runs(a, total);
-        if (my_run >= runs) return;
         const long long from = run_start(total, runs, my_run);
-        left = run_start(total, runs, my_run + 1) - from;
+        left = my_run < runs ? run_start(total, runs, my_run + 1) - from : 0;
+        if (tid == 0) {
+            // The unit that the run ends in, if it goes on, is the next run's too.
+            *step_link(a, my_run) = StepLink{-1, 0, 0, 0};
+        }
         if (left <= 0) return;
+        end = from + left;
+        all_chunks = total;
+        all_runs = runs;
         long long before = 0;
         for (int b0 = 0; b0 < a.rows.batch && before <= from; b0 += C::THREADS) {
             const int i = b0 + tid;
@@ -784,7 +802,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
         named_bar_sync(1, 32 * WARPS);
         if (*failed && a.cluster == 0) return;  // all of them
         const bool partial = !(c0 == 0 && c1 == s.chunks) && a.cluster == 0;
-        float* slot = partial ? step_slot<C>(a.ws, my_run, c0 == 0 ? 1 : 0) : nullptr;
+        float* slot = partial ? step_slot<C>(a, my_run, c0 == 0 ? 1 : 0) : nullptr;
+        if (partial && c0 == 0 && tid == 0)  // the run's last unit: it ends s.chunks - c1 chunks behind the run
+            *step_link(a, my_run) = StepLink{
+                static_cast<int>(((end + s.chunks - c1) * all_runs - 1) / all_chunks), s.q.first, row_count, head};
         for (int x = tid; x < row_count * (D / 4); x += WARPS * 32) {
             const int r = x / (D / 4), d = 4 * (x % (D / 4));
             float top = kNoMax;
@@ -836,52 +857,49 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
     }
 }
 
-// Joins the partial results of the units that more than one run shares, in a
-// fixed order: four threads of a row's float4 take every fourth run each and
-// are joined in shared memory.  A CTA has 256 / D rows of a unit (blockIdx.y).
-template <class C, bool BF16>
-__global__ void __launch_bounds__(256) k_kv4_join(const Kv4Attn a) {
-    constexpr int D = C::D, ROWS = C::ROWS, LANES = D / 4;
-    __shared__ long long sums[8];
-    __shared__ float4 part_v[4][256 / 4];
-    __shared__ float2 part_ml[4][256 / 4];
-    const int b = blockIdx.x / a.cache.heads, head = blockIdx.x - b * a.cache.heads;
-    const StepSeq s = step_seq<C>(a, b);
-    const int row0 = blockIdx.y * (64 / LANES);
-    if (s.chunks == 0 || row0 >= s.q.n * a.group) return;
-    long long sum = 0, sum_before = 0;
-    for (int i = threadIdx.x; i < a.rows.batch; i += blockDim.x) {
-        const long long w = step_seq<C>(a, i).total(a.cache.heads);
-        sum += w;
-        if (i < b) sum_before += w;
-    }
-    const long long total = block_sum(sum, sums), before = block_sum(sum_before, sums);
-    const int runs = step_runs(a, total);
-    const long long u0 = before + static_cast<long long>(head) * s.chunks, u1 = u0 + s.chunks;
-    const int r0 = static_cast<int>(((u0 + 1) * runs - 1) / total), r1 = static_cast<int>((u1 * runs - 1) / total);
-    if (r0 == r1) return;  // one run had all of it
-    grid_dep_wait();       // all above is the caller's; the partial results are the step kernel's
+// Joins the partial results that the four threads of a value hold (every
+// fourth each, in order) and stores the rows' values; the CTA's 256 threads
+// have 256 / D rows.
+template <bool BF16, int D>
+__device__ __forceinline__ void join_and_store(const Kv4Attn& a, bool valid, int first, int row, int head, int d,
+                                               float top, float l, float4 v) {
+    __shared__ float4 part_v[4][64];
+    __shared__ float2 part_ml[4][64];
     const int quarter = threadIdx.x / 64, item = threadIdx.x % 64;
-    const int r = row0 + item / LANES, d = 4 * (item % LANES);
-    const bool valid = r < s.q.n * a.group;
-    float top = kNoMax, l = 0.0f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (valid) {
-#pragma unroll 4
-        for (int i = r0 + quarter; i <= r1; i += 4) {
-            const float* slot = step_slot<C>(a.ws, i, i == r0 ? 1 : 0);
-            kv4_merge(top, l, v, slot[ROWS * D + r], slot[ROWS * D + ROWS + r],
-                      *reinterpret_cast<const float4*>(slot + r * D + d));
-        }
-    }
     part_v[quarter][item] = v;
     part_ml[quarter][item] = make_float2(top, l);
     __syncthreads();
     if (quarter == 0 && valid) {
 #pragma unroll
         for (int k = 1; k < 4; ++k) kv4_merge(top, l, v, part_ml[k][item].x, part_ml[k][item].y, part_v[k][item]);
-        kv4_store_row<BF16, D>(a, s.q.first, r, head, d, v, top, l);
+        kv4_store_row<BF16, D>(a, first, row, head, d, v, top, l);
     }
+}
+
+// Joins the partial results of the units that more than one run shares.  The
+// CTA of the run that a unit begins in follows the link that the run left;
+// blockIdx.y takes 256 / D rows.
+template <class C, bool BF16>
+__global__ void __launch_bounds__(256) k_kv4_join(const Kv4Attn a) {
+    constexpr int D = C::D, ROWS = C::ROWS, LANES = D / 4;
+    grid_dep_wait();
+    const int run = blockIdx.x;
+    const StepLink link = *step_link(a, run);
+    const int quarter = threadIdx.x / 64, item = threadIdx.x % 64;
+    const int r = blockIdx.y * (64 / LANES) + item / LANES, d = 4 * (item % LANES);
+    if (link.last < 0 || static_cast<int>(blockIdx.y) * (64 / LANES) >= link.rows) return;
+    const bool valid = r < link.rows;
+    float top = kNoMax, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (valid) {
+#pragma unroll 4
+        for (int i = run + quarter; i <= link.last; i += 4) {
+            const float* slot = step_slot<C>(a, i, i == run ? 1 : 0);
+            kv4_merge(top, l, v, slot[ROWS * D + r], slot[ROWS * D + ROWS + r],
+                      *reinterpret_cast<const float4*>(slot + r * D + d));
+        }
+    }
+    join_and_store<BF16, D>(a, valid, link.first, r, link.head, d, top, l, v);
 }
 
 }  // namespace tb
