@@ -184,6 +184,7 @@ AttnPlan plan_attention(int batch, int heads, int dim, int page_shift, int group
         // Fewer units than SMs: a unit's tokens are shared, 512 at least to each.
         const long long items = units * p.prompt_tiles;
         p.splits = static_cast<int>(std::max(1ll, std::min(sms / std::max(items, 1ll), max_len / 512ll)));
+        p.bytes += 16;  // the items' counter
         if (p.splits > 1)
             p.bytes += static_cast<size_t>(items) * p.splits * kPromptRows * (dim + 2) * sizeof(float);
     }
@@ -255,25 +256,32 @@ cudaError_t run_step(const Kv4Attn& a, cudaStream_t st) {
 }
 
 template <int D, bool BF16>
-cudaError_t run_prompt(const Kv4Attn& a, int sms, cudaStream_t st) {
+cudaError_t run_prompt(const Kv4Attn& a, int max_rows, int sms, cudaStream_t st) {
     using C = PromptCfg<D>;
-    static std::atomic<uint64_t> done{0};
-    cudaError_t e = prepare_kernel(k_kv4_prompt<C, BF16>, C::SMEM, C::REGS, done);
+    // Items drawn from a counter where fewer than three quarters of batch *
+    // max_rows rows are there, so that sequences are unlike; else a fixed share
+    // each.  32 heads of 128, 8 KV heads, drawn against fixed: 3 prompts of 2048
+    // and 13 single rows 209, 279 us; 2048 rows behind 2048 tokens and 63 single
+    // rows 304, 351 us; but 8 prompts of 2000 468, 445 us, one of 4096 171, 162 us.
+    const bool drawn = a.rows.rows * 4ll < static_cast<long long>(a.rows.batch) * max_rows * 3;
+    const auto kernel = drawn ? k_kv4_prompt<C, BF16, true> : k_kv4_prompt<C, BF16, false>;
+    static std::atomic<uint64_t> done[2] = {};
+    cudaError_t e = prepare_kernel(kernel, C::SMEM, C::REGS, done[drawn]);
     if (e != cudaSuccess) return e;
     const int ctas = std::min(a.prompt_units * a.prompt_splits, sms);
-    e = launch_early(k_kv4_prompt<C, BF16>, dim3(ctas), kPromptThreads, C::SMEM, st, a);
+    e = launch_early(kernel, dim3(ctas), kPromptThreads, C::SMEM, st, a);
     if (e != cudaSuccess || a.prompt_splits == 1) return e;
     k_kv4_prompt_join<C, BF16><<<dim3(a.prompt_units, kPromptRows * D / 256), 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 
 template <int D, bool BF16>
-cudaError_t run_attention(const Kv4Attn& a, int nt, int sms, cudaStream_t st) {
+cudaError_t run_attention(const Kv4Attn& a, int nt, int max_rows, int sms, cudaStream_t st) {
     if (nt == 1) return run_step<D, 1, BF16>(a, st);
     if (nt == 2) return run_step<D, 2, BF16>(a, st);
     if (nt == 3) return run_step<D, 3, BF16>(a, st);
     const cudaError_t e = run_step<D, 4, BF16>(a, st);
-    return e == cudaSuccess && a.prompt_tiles ? run_prompt<D, BF16>(a, sms, st) : e;
+    return e == cudaSuccess && a.prompt_tiles ? run_prompt<D, BF16>(a, max_rows, sms, st) : e;
 }
 
 tb_status check_heads(const tb_kv4_cache* c, int q_heads, int max_rows, int max_len) {
@@ -371,8 +379,8 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     int sms = 0;
     s = check_gpu(&sms);
     if (s != TB_OK) return s;
-    const AttnPlan p = plan_attention(a.rows.batch, a.cache.heads, a.cache.dim, a.cache.page_shift, a.group,
-                                      std::min(max_rows, a.rows.rows), max_len, window, sinks, sms);
+    max_rows = std::min(max_rows, a.rows.rows);
+    const AttnPlan p = plan_attention(a.rows.batch, a.cache.heads, a.cache.dim, a.cache.page_shift, a.group, max_rows, max_len, window, sinks, sms);
     if (p.bytes) {
         if (!workspace || workspace_bytes < p.bytes) return refuse(TB_ERR_WORKSPACE, "workspace missing or too small");
         if (!aligned16(workspace)) return refuse(TB_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
@@ -382,7 +390,8 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     a.runs = p.runs;
     a.min_run = p.min_run;
     a.step_rows = 8 * p.nt;
-    a.prompt_ws = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.step_bytes);
+    a.ticket = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + p.step_bytes);
+    a.prompt_ws = reinterpret_cast<float*>(a.ticket + 4);
     a.prompt_tiles = p.prompt_tiles;
     a.prompt_splits = p.splits;
     const long long units = static_cast<long long>(a.rows.batch) * a.cache.heads * std::max(p.prompt_tiles, 1);
@@ -391,8 +400,10 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     a.prompt_units = static_cast<int>(units);
     const bool bf16 = fmt == TB_FMT_BF16;
     cudaError_t e;
-    if (a.cache.dim == 128) e = bf16 ? run_attention<128, true>(a, p.nt, sms, stream) : run_attention<128, false>(a, p.nt, sms, stream);
-    else e = bf16 ? run_attention<64, true>(a, p.nt, sms, stream) : run_attention<64, false>(a, p.nt, sms, stream);
+    if (a.cache.dim == 128)
+        e = bf16 ? run_attention<128, true>(a, p.nt, max_rows, sms, stream) : run_attention<128, false>(a, p.nt, max_rows, sms, stream);
+    else
+        e = bf16 ? run_attention<64, true>(a, p.nt, max_rows, sms, stream) : run_attention<64, false>(a, p.nt, max_rows, sms, stream);
     return launched(e);
 }
 

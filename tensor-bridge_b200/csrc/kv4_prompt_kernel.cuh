@@ -1,8 +1,11 @@
 // kv4_prompt_kernel.cuh -- attention of many rows per sequence (a prompt, or a
 // chunk of one) over the block-scaled FP4 cache, on tcgen05.
 //
-// The kernel is persistent: a CTA takes an item of each round, and what loads
-// and decodes goes on into the next one while the last rows are finished.
+// The kernel is persistent, and what loads and decodes goes on into the next
+// item while the last one's rows are finished.  Where the sequences have like
+// numbers of rows a CTA takes an item of each round.  Else (DRAWN) the loading
+// warp draws items from a counter that all CTAs share and hands their numbers
+// on through a ring.
 // An item is 256 packed rows (token, head of one KV head's group) as two tiles
 // of 128 and runs over their visible tokens in tiles of 128:
 //   S_t = Q_t K^T     tcgen05.mma, both operands in shared memory, S_t in TMEM
@@ -36,6 +39,7 @@ namespace tb {
 
 constexpr int kPromptRows = 256;
 constexpr int kPromptTile = 128;                    // tokens
+constexpr int kPromptBatch = 2048;                  // sequences that a list of those with rows here holds
 constexpr int kPromptThreads = 640;                 // warps: 8 softmax, 4 decode K, 4 decode V, MMA, loader, 2 idle
 
 template <int D_>
@@ -51,8 +55,10 @@ struct PromptCfg {
     static constexpr int OFF_SLOT = 2 * OPERAND;
     static constexpr int OFF_RAW = OFF_SLOT + SLOTS * OPERAND;
     static constexpr int OFF_BAR = OFF_RAW + NR * RAW;
-    static constexpr int OFF_QSCALE = OFF_BAR + 256;
-    static constexpr int SMEM = OFF_QSCALE + kPromptRows * 4 + 1024;  // + alignment of the base
+    static constexpr int OFF_QSCALE = OFF_BAR + 512;
+    static constexpr int OFF_LIST = OFF_QSCALE + kPromptRows * 4;
+    static constexpr int SMEM = OFF_LIST + kPromptBatch * 4 + 1024;  // + alignment of the base
+    static_assert(SMEM <= 227 * 1024, "shared memory");
     static constexpr int S_COLS = 128;
     static constexpr int O_COL = 256;
     // Registers a thread: at launch, then by role.
@@ -60,13 +66,6 @@ struct PromptCfg {
     static_assert(256 * (REGS_SOFTMAX + REGS_DECODE) + 128 * REGS_REST <= kPromptThreads * REGS, "registers of the launch");
     static constexpr int SLOT_FLOATS = kPromptRows * (D + 2);
 };
-
-// The CTA's item of round r: there and back through the items, which come
-// largest first, so that the sums are alike.
-__device__ __forceinline__ int prompt_item(int r) {
-    return r * static_cast<int>(gridDim.x) +
-           static_cast<int>(r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-}
 
 // Low word of the descriptor of an N-major operand tile (V as [token][d]): 64
 // values of N are a 128-byte row, 8 rows of K an atom of 1024 bytes (the stride
@@ -92,21 +91,15 @@ struct PromptUnit {
     int first_pos, last_pos;
     int t0, t1;  // tiles of the span
     bool any;
+    int split;  // share of its tokens
 };
 
-__device__ __forceinline__ PromptUnit prompt_unit(const Kv4Attn& a, int item) {
+// Row tile `tile` of KV head `head` of sequence b, with all its tokens.
+__device__ __forceinline__ PromptUnit prompt_rows(const Kv4Attn& a, int b, int head, int tile) {
     PromptUnit u;
-    int unit = item, split = 0;
-    if (a.prompt_splits > 1) {
-        unit = item / a.prompt_splits;
-        split = item - unit * a.prompt_splits;
-    }
-    // The last row tiles see the most tokens: they come first.
-    const int per_tile = a.rows.batch * a.cache.heads;
-    const int tile = a.prompt_tiles - 1 - unit / per_tile;
-    const int rest = unit % per_tile;
-    u.b = rest / a.cache.heads;
-    u.head = rest - u.b * a.cache.heads;
+    u.b = b;
+    u.head = head;
+    u.split = 0;
     u.q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[u.b], a.rows.cu[u.b + 1], a.rows.lens[u.b]);
     u.row_base = tile * kPromptRows;
     u.row_count = min(kPromptRows, u.q.n * a.group - u.row_base);
@@ -117,8 +110,37 @@ __device__ __forceinline__ PromptUnit prompt_unit(const Kv4Attn& a, int item) {
     u.last_pos = u.q.pos0 + (u.row_base + u.row_count - 1) / a.group;
     u.span = kv4_span(u.first_pos, u.last_pos, u.q.len, a.window, a.sinks, 7);
     u.t1 = kv4_span_chunks(u.span);
+    return u;
+}
+
+// Where the partial results of a unit's share lie.
+template <class C>
+__device__ __forceinline__ float* prompt_slot(const Kv4Attn& a, const PromptUnit& u, int split) {
+    const size_t unit = (static_cast<size_t>(u.b) * a.prompt_tiles + u.row_base / kPromptRows) * a.cache.heads + u.head;
+    return a.prompt_ws + (unit * a.prompt_splits + split) * C::SLOT_FLOATS;
+}
+
+// Item number `item`: share (item % splits) of unit item / splits.  A unit is a
+// KV head of a row tile; a sequence's last row tiles see the most tokens, so all
+// sequences' last ones come first.  `list` holds the `seqs` sequences that have
+// row tiles here; nullptr: all of them.
+__device__ __forceinline__ PromptUnit prompt_unit(const Kv4Attn& a, const int* list, int seqs, int item) {
+    PromptUnit u;
+    int unit = item, split = 0;
+    if (a.prompt_splits > 1) {
+        unit = item / a.prompt_splits;
+        split = item - unit * a.prompt_splits;
+    }
+    const int per_tile = seqs * a.cache.heads;
+    const int tile = a.prompt_tiles - 1 - unit / per_tile;
+    const int rest = unit % per_tile;
+    u.b = rest / a.cache.heads;
+    u.head = rest - u.b * a.cache.heads;
+    if (list != nullptr) u.b = list[u.b];
+    u = prompt_rows(a, u.b, u.head, tile);
     if (a.prompt_splits > 1) {
         const long long tiles = u.t1;
+        u.split = split;
         u.t0 = static_cast<int>(tiles * split / a.prompt_splits);
         u.t1 = static_cast<int>(tiles * (split + 1) / a.prompt_splits);
     }
@@ -297,7 +319,7 @@ __device__ __forceinline__ PromptRow prompt_row(const Kv4Attn& a, const PromptUn
     return p;
 }
 
-template <class C, bool BF16>
+template <class C, bool BF16, bool DRAWN>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn a) {
     constexpr int D = C::D;
     extern __shared__ uint8_t smem_raw[];
@@ -312,9 +334,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
     uint64_t* o_full = pv_half + 2;
     uint64_t* q_full = o_full + 2;
     uint64_t* drain = q_full + 2;
-    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* item_full = drain + 1;         // a ring of four item numbers
+    uint64_t* item_empty = item_full + 4;
+    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(item_empty + 4);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-    volatile int* nan_seen = abort + 1;  // [round & 3]: the item whose V had a NaN block left out
+    volatile int* nan_seen = abort + 1;  // some item's V had a NaN block left out
+    volatile int* ring = nan_seen + 1;   // items by round & 3, -1 behind the last
+    int* warp_sums = const_cast<int*>(ring) + 4;  // 20
     float* q_scale = reinterpret_cast<float*>(smem + C::OFF_QSCALE);  // score -> log2 units, per row
 
     // A value that a shuffle or a vote gives is the same in the whole warp for
@@ -339,9 +365,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             mbar_init(&q_full[i], 4);
         }
         mbar_init(drain, 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&item_full[i], 1);
+            mbar_init(&item_empty[i], 17);
+        }
         fence_barrier_init();
         *abort = 0;
-        for (int i = 0; i < 4; ++i) nan_seen[i] = -1;
+        *nan_seen = 0;
     }
     if (warp == 16) tmem_alloc(tmem_ptr, 512);
     tc_fence_before();
@@ -349,8 +379,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
     tc_fence_after();
     const uint32_t tmem = *tmem_ptr;
 
-    const int items = a.prompt_units * a.prompt_splits;
-    const int rounds = (items + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    int seqs = a.rows.batch;
+    int* list = nullptr;
+    if (DRAWN && a.rows.batch <= kPromptBatch) {  // more do not fit: then all are gone through
+        list = reinterpret_cast<int*>(smem + C::OFF_LIST);
+        seqs = 0;
+        for (int b0 = 0; b0 < a.rows.batch; b0 += kPromptThreads) {
+            const int b = b0 + tid;
+            const bool here = b < a.rows.batch && prompt_takes(a, kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[b],
+                                                                          a.rows.cu[b + 1], a.rows.lens[b]));
+            const uint32_t some = __ballot_sync(0xFFFFFFFFu, here);
+            if (lane == 0) warp_sums[warp] = __popc(some);
+            __syncthreads();
+            int before = seqs + __popc(some & ((1u << lane) - 1u));
+            for (int k = 0; k < kPromptThreads / 32; ++k) {
+                if (k < warp) before += warp_sums[k];
+                seqs += warp_sums[k];
+            }
+            if (here) list[before] = b;
+            __syncthreads();
+        }
+    }
+    const int items = seqs * a.cache.heads * a.prompt_tiles * a.prompt_splits;
+    // The next item (-1: none); `round` counts those that the warp has had.
+    uint32_t round = 0;
+    auto take_item = [&]() {
+        int item = -1;
+        if constexpr (DRAWN) {
+            if (__all_sync(0xFFFFFFFFu, mbar_wait(&item_full[round & 3], (round >> 2) & 1, abort))) {
+                item = ring[round & 3];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&item_empty[round & 3]);
+            }
+        } else {  // there and back through the items, so that the CTAs' sums are alike
+            item = static_cast<int>(round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
+            if (item >= items) item = -1;
+        }
+        ++round;
+        return item;
+    };
+
     const int gshift = a.cache.page_shift < 7 ? a.cache.page_shift : 7;
     const uint32_t gtok = 1u << gshift;
     const uint32_t at_ks = gtok * (D / 2), at_vc = at_ks + gtok * (D / 16), at_vs = at_vc + gtok * (D / 2);
@@ -367,15 +435,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         bool ok = true;
         const int warp_row = (warp & 3) * 32;  // first of the warp's rows in the tile
         uint8_t* q_tile = smem + t * C::OPERAND;
-        // The next round with rows for this tile, from `round` on.
-        auto find = [&](int round, PromptUnit& u) {
-            for (; round < rounds; ++round) {
-                const int item = prompt_item(round);
-                if (item >= items) return rounds;  // only in the last round
-                u = prompt_unit(a, item);
-                if (u.t0 < u.t1 && u.row_count > t * 128) break;
+        // The next item with rows for this tile; -1: none.
+        auto find = [&](PromptUnit& u) {
+            for (;;) {
+                const int item = take_item();
+                if (item < 0) return -1;
+                u = prompt_unit(a, list, seqs, item);
+                if (u.t0 < u.t1 && u.row_count > t * 128) return item;
             }
-            return round;
         };
         auto give_q = [&](const PromptQ<C>& q) {
             prompt_q_store<C, BF16>(a, q, q_tile, warp_row, q_scale + t * 128);
@@ -384,14 +451,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             if (lane == 0) mbar_arrive(&q_full[t]);
         };
         PromptUnit u;
-        int round = find(0, u);
-        if (round < rounds) {
+        int item = find(u);
+        if (item >= 0) {
             PromptQ<C> q;
             prompt_q_load<C>(a, u, t * 128 + warp_row, q);
             give_q(q);
         }
-        while (round < rounds && ok) {
-            const int item = prompt_item(round);
+        while (item >= 0 && ok) {
             const PromptRow row = prompt_row(a, u, t * 128 + r);
             const int pos = row.pos;
             const float f = q_scale[t * 128 + r];  // written by this warp
@@ -475,13 +541,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
 
             // ---- the rows' result ----------------------------------------------------------
             PromptUnit un;
-            const int round_next = find(round + 1, un);
+            const int item_next = find(un);
             ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&o_full[t], o_phase, abort));
             o_phase ^= 1u;
             if (!ok) break;
             tc_fence_after();
             uint32_t nan_blocks = 0;
-            if (nan_seen[round & 3] == item && row.valid) {
+            if (*nan_seen && row.valid) {
                 // Rare: look at every block of V that was left out of a
                 // partly visible tile, and put a NaN where this row sees it.
                 for (int j = u.t0; j < u.t1; ++j) {
@@ -505,7 +571,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             // products have ended), D / 8 chunks of 16 bytes of a row at a time,
             // chunk x at x ^ (row & 7) of its panel, so that they leave in whole
             // lines: with a row a thread this took 5 us an item.
-            float* slot = a.prompt_ws + static_cast<size_t>(item) * C::SLOT_FLOATS;
+            float* slot = prompt_slot<C>(a, u, u.split);
             uint8_t* stage = q_tile + warp_row * 128;
             uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(u.head) * a.group * D +
                             8 * (lane % PromptQ<C>::LANES);
@@ -580,7 +646,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                 __syncwarp();
             }
             PromptQ<C> q;
-            if (round_next < rounds) prompt_q_load<C>(a, un, t * 128 + warp_row, q);
+            if (item_next >= 0) prompt_q_load<C>(a, un, t * 128 + warp_row, q);
             if (row.valid && partial) {
                 slot[kPromptRows * D + t * 128 + r] = m;
                 slot[kPromptRows * (D + 1) + t * 128 + r] = l;
@@ -589,9 +655,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
             }
             tc_fence_before();  // O has been read before the next item's P is announced
-            if (round_next < rounds) give_q(q);
+            if (item_next >= 0) give_q(q);
             u = un;
-            round = round_next;
+            item = item_next;
         }
     } else if (warp < 16) {
         reg_dec<C::REGS_DECODE>();
@@ -602,10 +668,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         int rs = 0, slot = 0;
         uint32_t r_phase = 0, op_phase = 1;  // of the empty slot: the first round passes at once
         bool ok = true;
-        for (int round = 0; round < rounds && ok; ++round) {
-            const int item = prompt_item(round);
-            if (item >= items) break;  // only in the last round
-            const PromptUnit u = prompt_unit(a, item);
+        for (int item = take_item(); item >= 0 && ok; item = take_item()) {
+            const PromptUnit u = prompt_unit(a, list, seqs, item);
             int page = prompt_look(a, u, u.t0);
             for (int j = u.t0; j < u.t1; ++j) {
                 const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
@@ -633,7 +697,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     if (kv && !open && e4m3_nan_bits(sc)) {
                         // A NaN block that some row may not see: out of the
                         // product, and into the rows that see it at the end.
-                        nan_seen[round & 3] = item;
+                        *nan_seen = 1;
                         __threadfence_block();
                         sc &= ~((e4m3_nan_bits(sc) >> 7) * 0xFFu);
                     }
@@ -713,10 +777,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         auto next = [&]() {
             if (++slot == C::SLOTS) slot = 0, op_phase ^= 1u;
         };
-        for (int round = 0; round < rounds && ok; ++round) {
-            const int item = prompt_item(round);
-            if (item >= items) break;  // only in the last round
-            const PromptUnit u = prompt_unit(a, item);
+        for (int item = take_item(); item >= 0 && ok; item = take_item()) {
+            const PromptUnit u = prompt_unit(a, list, seqs, item);
             const int n = __reduce_max_sync(0xFFFFFFFFu, u.t1 - u.t0);
             if (n == 0) continue;
             const bool two = __any_sync(0xFFFFFFFFu, u.row_count > 128);
@@ -795,15 +857,42 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         int rs = 0;
         uint32_t r_phase = 1, filled = 0;  // of the empty stage: the first round passes at once
         bool ok = true;
-        for (int round = 0; round < rounds && ok; ++round) {
-            const int item = prompt_item(round);
-            if (item >= items) break;  // only in the last round
-            const PromptUnit u = prompt_unit(a, item);
+        // The first item is the CTA's own, later ones are drawn from the
+        // counter, which the step kernel set to 0.
+        auto draw = [&](int item) {
+            if constexpr (DRAWN) {
+                if (item < 0) {
+                    item = blockIdx.x;
+                } else {
+                    if (round < 2) grid_dep_wait();
+                    if (lane == 0) item = static_cast<int>(gridDim.x) + atomicAdd(a.ticket, 1);
+                    item = __shfl_sync(0xFFFFFFFFu, item, 0);
+                }
+                return item < items ? item : -1;
+            } else {
+                return take_item();
+            }
+        };
+        auto publish = [&](int item) {
+            if constexpr (DRAWN) {
+                ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&item_empty[round & 3], ((round >> 2) & 1) ^ 1u, abort));
+                if (lane == 0 && ok) {
+                    ring[round & 3] = item;
+                    mbar_arrive(&item_full[round & 3]);
+                }
+                __syncwarp();
+                ++round;
+            }
+        };
+        for (int item = draw(-1); item >= 0 && ok; item = draw(item)) {
+            const PromptUnit u = prompt_unit(a, list, seqs, item);
             if (lane == 0 && u.any) {
                 if (u.q.bad) atomicOr(&g_tb_device_error, kErrPage);
                 if (static_cast<long long>(u.q.n) * a.group > static_cast<long long>(a.prompt_tiles) * kPromptRows)
                     atomicOr(&g_tb_device_error, kErrRows);
             }
+            if (u.t0 == u.t1) continue;
+            publish(item);
             int after = prompt_look(a, u, u.t0);
             for (int j = u.t0; j < u.t1; ++j) {
                 const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
@@ -838,6 +927,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                 if (++rs == C::NR) rs = 0, r_phase ^= 1u;
             }
         }
+        publish(-1);
         if (!ok && lane == 0)  // copies in flight end before the memory is given up
             for (int k = 0; k < C::NR && filled > 0; ++k, --filled) {
                 if (--rs < 0) rs = C::NR - 1, r_phase ^= 1u;
@@ -861,19 +951,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
 template <class C, bool BF16>
 __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4Attn a) {
     constexpr int D = C::D, LANES = D / 4;
-    const PromptUnit u = prompt_unit(a, blockIdx.x * a.prompt_splits);
+    const int per = a.cache.heads * a.prompt_tiles, b = blockIdx.x / per, tile = blockIdx.x % a.prompt_tiles;
     const int quarter = threadIdx.x / 64, item = threadIdx.x % 64;
     const int r = blockIdx.y * (64 / LANES) + item / LANES, d = 4 * (item % LANES);
+    const PromptUnit u = prompt_rows(a, b, (blockIdx.x - b * per) / a.prompt_tiles, tile);
     if (!u.any || static_cast<int>(blockIdx.y) * (64 / LANES) >= u.row_count) return;
     const bool valid = r < u.row_count;
-    const long long tiles = kv4_span_chunks(u.span);
+    const long long tiles = u.t1;
     float top = kNoMax, l = 0.0f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (valid) {
 #pragma unroll 4
         for (int s = quarter; s < a.prompt_splits; s += 4) {
             if (tiles * s / a.prompt_splits == tiles * (s + 1) / a.prompt_splits) continue;  // no tiles, no result
-            const float* slot = a.prompt_ws + (static_cast<size_t>(blockIdx.x) * a.prompt_splits + s) * C::SLOT_FLOATS;
+            const float* slot = prompt_slot<C>(a, u, s);
             kv4_merge(top, l, v, slot[kPromptRows * D + r], slot[kPromptRows * (D + 1) + r],
                       *reinterpret_cast<const float4*>(slot + r * D + d));
         }

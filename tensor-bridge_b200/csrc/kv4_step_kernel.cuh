@@ -61,6 +61,7 @@ struct Kv4Attn {
     int min_run;                   // chunks a CTA should have at least
     int step_rows;                 // packed rows that the step kernel takes; sequences with more are the prompt kernel's
     float* prompt_ws;
+    int* ticket;                   // counter of the prompt kernel's items, set to 0 by the step kernel
     int prompt_tiles;              // tiles of 256 packed rows of a sequence at most
     int prompt_splits;             // CTAs that share a prompt unit's tokens
     int prompt_units;              // sequences * KV heads * prompt_tiles
@@ -290,7 +291,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
 
     volatile int* failed = abort + 1;  // by a computing warp, before its second barrier of a unit
 
-    grid_dep_launch_dependents();  // k_kv4_join waits for this grid's end
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.prompt_tiles > 0) *a.ticket = 0;
+    grid_dep_launch_dependents();  // what comes next waits for this grid's end
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     const int g = lane >> 2, c = lane & 3;
     if (tid == 0) {

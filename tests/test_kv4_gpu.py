@@ -141,9 +141,9 @@ class Batch:
             assert np.all(ls[self.cu[-1]:] == 7.0)
 
     def run(self, q_heads, scale=None, std=1.0, **kw):
-        scale = self.host.dim ** -0.5 if scale is None else scale
         """Both ways of sharing a sequence: short (clusters) and long (runs of
         chunks), chosen by max_len."""
+        scale = self.host.dim ** -0.5 if scale is None else scale
         q, dense = self.queries(q_heads, std)
         for max_len in (kw.pop("max_len", None), LONG):
             out, lse = self.attend(q, q_heads, scale, max_len=max_len, **kw)
@@ -390,6 +390,45 @@ def test_long_prompt(tb, cuda, page, dim):
     bt = Batch(tb, cuda, [1500], [700], page=page, heads=1, dim=dim, typ="bf16", seed=2)
     bt.fill_fast()
     bt.run(2)
+
+
+@pytest.mark.parametrize("batch", [40, 700, 2100])
+def test_unlike_sequences(tb, cuda, batch):
+    """Many single rows, some idle sequences, and prompts of one to several row
+    tiles among them, the first and the last included."""
+    n = [1 if b % 9 else 0 for b in range(batch)]
+    lens = [5 + b % 40 for b in range(batch)]
+    for b, rows, length in ((0, 40, 50), (7, 600, 600), (8, 130, 700), (batch // 2, 9, 300), (batch - 1, 300, 310)):
+        n[b], lens[b] = rows, length
+    bt = Batch(tb, cuda, lens, n, page=32, heads=1, dim=64, typ="bf16", seed=batch, pad=2)
+    bt.fill_fast()
+    bt.run(4)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_cache_of_many_gigabytes(tb, cuda, n):
+    """Pages 700 MB apart, so that offsets pass 32 bits: written, read, attended."""
+    apart = 700 * 2 ** 20
+    bt = Batch(tb, cuda, [70 + n, 90], [n, n], page=16, heads=2, dim=64, seed=80 + n, spare=0)
+    bt.fill()
+    far = cuda.empty((bt.host.pages, apart), dtype=cuda.uint8, device="cuda")
+    size = bt.host.stride
+    small = cuda.from_numpy(bt.host.data[:, :size].copy()).cuda()
+    assert far.numel() > 2 ** 32
+    far[:, :size] = small
+    far[:, size:size + 4096] = 0xA5
+    bt.cache = tb.KV4Cache(far, bt.host.pages, 16, 2, 64, bt.host.k_scale, bt.host.v_scale, apart)
+    bt.run(8)
+    val, words = to_bits(bt.rng.normal(size=(bt.total, 2, 2, 64)).astype(np.float32), "f16")
+    kv = cuda.from_numpy(words).cuda()
+    tb.kv4_append(bt.cache, bt.rows, tb.Format.F16, kv.data_ptr(), kv.data_ptr() + 256, k_stride=256, v_stride=256)
+    for b in range(2):
+        for i in range(n):
+            bt.host.write(*bt.place(b, bt.lens[b] - n + i), *val[bt.cu[b] + i])
+    assert np.array_equal(far[:, :size].cpu().numpy(), bt.host.data)
+    assert bool((far[:, size:size + 4096] == 0xA5).all())
+    read_and_compare(bt)
+    bt.run(8)
 
 
 @pytest.mark.parametrize("n", [33, 127, 128, 129, 255, 256, 257, 300])
@@ -644,6 +683,49 @@ def test_same_bits_again_and_in_a_graph(tb, cuda, n, max_len):
     # the eager call follows too
     out1, lse1 = bt.attend(q, 8, 0.09, max_len=max_len)
     assert cuda.equal(out, out1) and cuda.equal(lse, lse1)
+
+
+def test_generation_in_one_graph(tb, cuda):
+    """A step of a generation, captured once: a token written, then attended.
+    Each replay reads the lengths, the pages and the new values from the device."""
+    bt = Batch(tb, cuda, [31, 140], [1, 1], page=16, heads=2, dim=128, seed=90, spare=4)
+    bt.fill()
+    val, words = to_bits(bt.rng.normal(size=(3, 2, 2, 2, 128)).astype(np.float32), "f16")
+    kv = cuda.from_numpy(words[0].copy()).cuda()
+    q, _ = bt.queries(8)
+    out = cuda.full((2, 1024), 7.0, dtype=cuda.float16, device="cuda")
+    lse = cuda.full((2, 8), 7.0, dtype=cuda.float32, device="cuda")
+    need = tb.kv4_attention_workspace(bt.cache, bt.rows, 8, 1, LONG)
+    ws = cuda.full((need,), 0xFF, dtype=cuda.uint8, device="cuda")
+
+    def step(stream):
+        tb.kv4_append(bt.cache, bt.rows, tb.Format.F16, kv, kv.data_ptr() + 512, k_stride=512, v_stride=512, stream=stream)
+        tb.kv4_attention(bt.cache, bt.rows, tb.Format.F16, q, out, lse, 8, 1, LONG, 0.09, workspace=ws,
+                         workspace_bytes=need, stream=stream)
+
+    side = cuda.cuda.Stream()
+    graph = cuda.cuda.CUDAGraph()
+    cuda.cuda.synchronize()
+    with cuda.cuda.graph(graph, stream=side):
+        step(side)
+    free = [p for p in range(bt.host.pages) if p not in bt.table]
+    for i in range(3):
+        if i:
+            bt.lens = [x + 1 for x in bt.lens]
+            for b in range(2):
+                if (bt.lens[b] - 1) % 16 == 0:
+                    at = (bt.lens[b] - 1) // 16
+                    if at == bt.table.shape[1]:
+                        pytest.fail("the table is too narrow")
+                    bt.table[b, at] = free.pop()
+            bt.d_lens.copy_(cuda.tensor(bt.lens, dtype=cuda.int32))
+            bt.d_table.copy_(cuda.from_numpy(bt.table))
+            kv.copy_(cuda.from_numpy(words[i].copy()))
+        for b in range(2):
+            bt.host.write(*bt.place(b, bt.lens[b] - 1), *val[i, b])
+        graph.replay()
+        cuda.cuda.synchronize()
+        bt.check(out, lse, q, 8, 0.09)
 
 
 def test_streams_side_by_side(tb, cuda):
