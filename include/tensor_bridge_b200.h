@@ -330,6 +330,8 @@ typedef struct tb_kv4_cache {
  * cu_rows[batch] to `rows` belong to nobody (a padded batch): they are not
  * read and what would be written to them stays as it was.  Table entries
  * behind a sequence's last page are not read.
+ * Pages that a window hides from all of a sequence's rows may be gone: their
+ * entries may hold any number (another sequence's page, -1).
  * Contents that the host cannot check are checked on the device: a row whose
  * token number is negative or whose page is not in [0, num_pages) or not in
  * the table is left out (not written, not read back, not seen by attention;

@@ -16,6 +16,8 @@
 // are, where a search per row would be a chain of them), then a warp takes a
 // (K or V, head) pair and runs over the CTA's rows, so that tokens which are
 // neighbours in a page are read and written by neighbouring lanes.
+// Measured, 131072 rows of 8 KV heads of 128: append 139 us (4.96 TB/s, 0.76 of
+// a copy; with every border compared, 213 us), read 124 us (5.57 TB/s, 0.85).
 #pragma once
 
 #include <cuda_bf16.h>

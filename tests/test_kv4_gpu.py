@@ -508,12 +508,12 @@ def test_what_lies_behind_a_sequence_is_not_seen(tb, cuda, max_len, n):
 
 @pytest.mark.parametrize("max_len", [None, LONG])
 @pytest.mark.parametrize("where", ["k", "v"])
-@pytest.mark.parametrize("n", [1, 3, 40])
-def test_nan_tokens_reach_the_rows_that_see_them(tb, cuda, max_len, where, n):
+@pytest.mark.parametrize("n,others", [(1, 0), (3, 0), (40, 0), (40, 6)])
+def test_nan_tokens_reach_the_rows_that_see_them(tb, cuda, max_len, where, n, others):
     """A cached NaN block is seen or hidden like any other token."""
     window, sinks = 50, 2
     lens = [400, 1300]
-    bt = Batch(tb, cuda, lens, [n, n], page=16, heads=1, dim=128, seed=33)
+    bt = Batch(tb, cuda, lens + [30] * others, [n, n] + [1] * others, page=16, heads=1, dim=128, seed=33)
     bt.fill_fast()
     bad = {0: [1, 200, 345, 360, 399], 1: [0, 100, 1251]}  # positions
     for b, ps in bad.items():
@@ -607,6 +607,31 @@ def test_pages_outside_the_cache_are_not_seen(tb, cuda, max_len, n):
             assert np.all(np.abs(got - want[0]) <= t_out)
 
 
+@pytest.mark.parametrize("max_len", [None, LONG])
+@pytest.mark.parametrize("gone", ["none", "other"])
+@pytest.mark.parametrize("n,page", [(1, 16), (1, 64), (3, 32), (40, 16), (40, 32), (300, 16)])
+def test_pages_out_of_sight_may_be_gone(tb, cuda, max_len, gone, n, page):
+    """Entries of pages behind the window: no page, or one of NaN blocks that
+    another sequence holds.  The results stay and nothing is reported."""
+    window, sinks = 70, 5
+    lens = [1500, 777 + n]
+    bt = Batch(tb, cuda, lens, [n, n], page=page, heads=2, dim=64, seed=37, spare=1)
+    bt.fill_fast()
+    free = next(p for p in range(bt.host.pages) if p not in bt.table)
+    bt.host.data[free] = 0x7F
+    bt.upload()
+    q, _ = bt.queries(4)
+    want = bt.attend(q, 4, 0.1, window=window, sinks=sinks, max_len=max_len)
+    for b in range(2):
+        oldest = lens[b] - n - window + 1
+        for slot in range(-(-lens[b] // page)):
+            if slot * page >= sinks and (slot + 1) * page <= oldest:
+                bt.table[b, slot] = -1 if gone == "none" else free
+    bt.index()
+    got = bt.attend(q, 4, 0.1, window=window, sinks=sinks, max_len=max_len)
+    assert cuda.equal(got[0], want[0]) and cuda.equal(got[1], want[1])
+
+
 def test_lengths_outside_the_table(tb, cuda):
     """A length that passes the table or is negative: the error word, and rows
     of the other sequences as before."""
@@ -683,6 +708,22 @@ def test_same_bits_again_and_in_a_graph(tb, cuda, n, max_len):
     # the eager call follows too
     out1, lse1 = bt.attend(q, 8, 0.09, max_len=max_len)
     assert cuda.equal(out, out1) and cuda.equal(lse, lse1)
+
+
+@pytest.mark.parametrize("max_len", [None, LONG])
+@pytest.mark.parametrize("n", [1, 6, 40, 300])
+def test_out_over_the_queries(tb, cuda, max_len, n):
+    """out may be q itself."""
+    bt = Batch(tb, cuda, [n + 400, n + 20, 90], [n, n, 1], page=16, heads=2, dim=128, seed=95, pad=1)
+    bt.fill_fast()
+    q, _ = bt.queries(8)
+    out, lse = bt.attend(q, 8, 0.09, max_len=max_len)
+    need = tb.kv4_attention_workspace(bt.cache, bt.rows, 8, n, max_len or max(bt.lens))
+    ws = cuda.full((max(need, 16),), 0xFF, dtype=cuda.uint8, device="cuda")
+    both, lse2 = q.clone(), cuda.full_like(lse, 7.0)
+    tb.kv4_attention(bt.cache, bt.rows, tb.Format.F16, both, both, lse2, 8, n, max_len or max(bt.lens), 0.09,
+                     workspace=ws, workspace_bytes=need)
+    assert cuda.equal(both[:-1], out[:-1]) and cuda.equal(lse, lse2) and cuda.equal(both[-1], q[-1])
 
 
 def test_generation_in_one_graph(tb, cuda):
