@@ -115,11 +115,14 @@ tb_status check_copy(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_form
 
 // A CTA of few rows starts fastest and spreads a step's rows over the SMs; one
 // of many rows has enough loads in flight.  The change is made where the small
-// CTAs would be more than the SMs hold at once (8 of 256 threads each).
-bool many_rows(const Kv4Copy& a, int per_cta, int sms, unsigned* y) {
+// CTAs would come in more than `per_sm` an SM (8 are there at once).  8 KV heads
+// of 128, few against many: append 592 rows 3.1, 6.8 us, 2400 rows 6.2, 8.9, 16384
+// rows 29.3, 22.1; read 592 rows 2.9, 5.2 us, 2400 rows 6.7, 6.9, 16384 rows
+// 32.4, 19.4.
+bool many_rows(const Kv4Copy& a, int per_cta, int per_sm, int sms, unsigned* y) {
     const int pairs = 2 * a.cache.heads;
     *y = static_cast<unsigned>((pairs + kKv4CopyThreads / 32 - 1) / (kKv4CopyThreads / 32));
-    return static_cast<long long>((a.rows.rows + per_cta - 1) / per_cta) * *y > 8ll * sms;
+    return static_cast<long long>((a.rows.rows + per_cta - 1) / per_cta) * *y > static_cast<long long>(per_sm) * sms;
 }
 
 dim3 copy_grid(const Kv4Copy& a, int per_cta, unsigned y) {
@@ -129,7 +132,7 @@ dim3 copy_grid(const Kv4Copy& a, int per_cta, unsigned y) {
 template <bool BF16>
 cudaError_t run_append(const Kv4Copy& a, cudaStream_t st, int sms) {
     unsigned y;
-    if (many_rows(a, 4, sms, &y)) k_kv4_append<BF16, 32, 2><<<copy_grid(a, 32, y), kKv4CopyThreads, 0, st>>>(a);
+    if (many_rows(a, 4, 20, sms, &y)) k_kv4_append<BF16, 32, 2><<<copy_grid(a, 32, y), kKv4CopyThreads, 0, st>>>(a);
     else k_kv4_append<BF16, 4, 1><<<copy_grid(a, 4, y), kKv4CopyThreads, 0, st>>>(a);
     return cudaGetLastError();
 }
@@ -137,7 +140,7 @@ cudaError_t run_append(const Kv4Copy& a, cudaStream_t st, int sms) {
 template <bool BF16>
 cudaError_t run_read(const Kv4Copy& a, cudaStream_t st, int sms) {
     unsigned y;
-    if (many_rows(a, 4, sms, &y)) k_kv4_read<BF16, 32, 8><<<copy_grid(a, 32, y), kKv4CopyThreads, 0, st>>>(a);
+    if (many_rows(a, 4, 9, sms, &y)) k_kv4_read<BF16, 32, 8><<<copy_grid(a, 32, y), kKv4CopyThreads, 0, st>>>(a);
     else k_kv4_read<BF16, 4, 2><<<copy_grid(a, 4, y), kKv4CopyThreads, 0, st>>>(a);
     return cudaGetLastError();
 }
@@ -150,12 +153,13 @@ struct AttnPlan {
     int cluster, runs, min_run;
     size_t step_bytes;  // of its partial results
     int prompt_tiles;   // 0: no sequence has more rows than the step kernel takes
+    bool drawn;         // its items are drawn from a counter
     int splits;
     size_t bytes;       // of both kernels' partial results
 };
 
-AttnPlan plan_attention(int batch, int heads, int dim, int page_shift, int group, int max_rows, int max_len, int window,
-                        int sinks, int sms) {
+AttnPlan plan_attention(int batch, int heads, int dim, int page_shift, int group, int call_rows, int max_rows,
+                        int max_len, int window, int sinks, int sms) {
     AttnPlan p{};
     const long long rows = static_cast<long long>(max_rows) * group;
     // Tokens that a sequence's rows see at most.  A window can only lower it,
@@ -175,18 +179,31 @@ AttnPlan plan_attention(int batch, int heads, int dim, int page_shift, int group
     const long long share = std::min(std::min(8ll, room), std::max(1ll, (max_len + 255ll) / 256));
     if (share > 0 && max_len <= share * (units * share * 4 >= p.runs * 3ll ? 2560 : 1024))
         p.cluster = static_cast<int>(share);
+    // A run has 512 tokens at least: one row at 16384 tokens 15.3 us, 15.9 with
+    // 256, 17.3 with 1024.
     p.min_run = std::max(1, 512 >> step_gran(page_shift, p.nt == 2 ? 7 : 8));
     p.step_bytes = p.cluster ? 0 : static_cast<size_t>(p.runs) * (sizeof(StepLink) + 2 * (8 * p.nt) * (dim + 2) * sizeof(float));
     p.splits = 1;
     p.bytes = p.step_bytes;
     if (rows > kStepRowsMost) {
         p.prompt_tiles = static_cast<int>((rows + kPromptRows - 1) / kPromptRows);
-        // Fewer units than SMs: a unit's tokens are shared, 512 at least to each.
-        const long long items = units * p.prompt_tiles;
-        p.splits = static_cast<int>(std::max(1ll, std::min(sms / std::max(items, 1ll), max_len / 512ll)));
+        // Items drawn from a counter where fewer than three quarters of batch *
+        // max_rows rows are there, so that sequences are unlike; else a fixed share
+        // each.  32 heads of 128, 8 KV heads, drawn against fixed: 3 prompts of 2048
+        // and 13 single rows 209, 279 us; 2048 rows behind 2048 tokens and 63 single
+        // rows 304, 351 us; but 8 prompts of 2000 468, 445 us, one of 4096 171, 162 us.
+        p.drawn = call_rows * 4ll < static_cast<long long>(batch) * max_rows * 3;
+        // Fewer units than SMs: a unit's tokens are shared, 512 at least to each
+        // (128 rows behind 3968 tokens, 8 KV heads: 35.2 us, 36.5 with 256, 39.2
+        // with 1024).
+        // Unlike sequences have about as many units as their rows fill tiles: 128
+        // rows behind 32640 tokens and 31 single rows 594 us, 1032 without shares.
+        const long long tiles = p.drawn ? (static_cast<long long>(call_rows) * group + kPromptRows - 1) / kPromptRows
+                                        : static_cast<long long>(batch) * p.prompt_tiles;
+        p.splits = static_cast<int>(std::max(1ll, std::min(sms / std::max(tiles * heads, 1ll), max_len / 512ll)));
         p.bytes += 16;  // the items' counter
         if (p.splits > 1)
-            p.bytes += static_cast<size_t>(items) * p.splits * kPromptRows * (dim + 2) * sizeof(float);
+            p.bytes += static_cast<size_t>(p.splits) * heads * call_rows * group * (dim + 2) * sizeof(float);
     }
     return p;
 }
@@ -256,14 +273,8 @@ cudaError_t run_step(const Kv4Attn& a, cudaStream_t st) {
 }
 
 template <int D, bool BF16>
-cudaError_t run_prompt(const Kv4Attn& a, int max_rows, int sms, cudaStream_t st) {
+cudaError_t run_prompt(const Kv4Attn& a, bool drawn, int sms, cudaStream_t st) {
     using C = PromptCfg<D>;
-    // Items drawn from a counter where fewer than three quarters of batch *
-    // max_rows rows are there, so that sequences are unlike; else a fixed share
-    // each.  32 heads of 128, 8 KV heads, drawn against fixed: 3 prompts of 2048
-    // and 13 single rows 209, 279 us; 2048 rows behind 2048 tokens and 63 single
-    // rows 304, 351 us; but 8 prompts of 2000 468, 445 us, one of 4096 171, 162 us.
-    const bool drawn = a.rows.rows * 4ll < static_cast<long long>(a.rows.batch) * max_rows * 3;
     const auto kernel = drawn ? k_kv4_prompt<C, BF16, true> : k_kv4_prompt<C, BF16, false>;
     static std::atomic<uint64_t> done[2] = {};
     cudaError_t e = prepare_kernel(kernel, C::SMEM, C::REGS, done[drawn]);
@@ -271,17 +282,19 @@ cudaError_t run_prompt(const Kv4Attn& a, int max_rows, int sms, cudaStream_t st)
     const int ctas = std::min(a.prompt_units * a.prompt_splits, sms);
     e = launch_early(kernel, dim3(ctas), kPromptThreads, C::SMEM, st, a);
     if (e != cudaSuccess || a.prompt_splits == 1) return e;
-    k_kv4_prompt_join<C, BF16><<<dim3(a.prompt_units, kPromptRows * D / 256), 256, 0, st>>>(a);
+    constexpr int kJoinRows = 256 / D;  // rows of a CTA of k_kv4_prompt_join
+    const unsigned x = static_cast<unsigned>((a.rows.rows * a.group + kJoinRows - 1) / kJoinRows);
+    k_kv4_prompt_join<C, BF16><<<dim3(x, a.cache.heads), 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 
 template <int D, bool BF16>
-cudaError_t run_attention(const Kv4Attn& a, int nt, int max_rows, int sms, cudaStream_t st) {
+cudaError_t run_attention(const Kv4Attn& a, int nt, bool drawn, int sms, cudaStream_t st) {
     if (nt == 1) return run_step<D, 1, BF16>(a, st);
     if (nt == 2) return run_step<D, 2, BF16>(a, st);
     if (nt == 3) return run_step<D, 3, BF16>(a, st);
     const cudaError_t e = run_step<D, 4, BF16>(a, st);
-    return e == cudaSuccess && a.prompt_tiles ? run_prompt<D, BF16>(a, max_rows, sms, st) : e;
+    return e == cudaSuccess && a.prompt_tiles ? run_prompt<D, BF16>(a, drawn, sms, st) : e;
 }
 
 tb_status check_heads(const tb_kv4_cache* c, int q_heads, int max_rows, int max_len) {
@@ -340,8 +353,8 @@ size_t tb_kv4_attention_workspace(const tb_kv4_cache* cache, const tb_kv4_rows* 
     Kv4Rows r{};
     if (check_cache(cache, &c) != TB_OK || check_rows(rows, c.page_shift, &r) != TB_OK) return 0;
     if (check_heads(cache, q_heads, max_rows, max_len) != TB_OK) return 0;
-    return plan_attention(r.batch, c.heads, c.dim, c.page_shift, q_heads / c.heads, std::min(max_rows, r.rows), max_len, 0, 0,
-                          device_info(current_device()).sms)
+    return plan_attention(r.batch, c.heads, c.dim, c.page_shift, q_heads / c.heads, r.rows,
+                          std::min(max_rows, r.rows), max_len, 0, 0, device_info(current_device()).sms)
         .bytes;
 }
 
@@ -380,7 +393,8 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     s = check_gpu(&sms);
     if (s != TB_OK) return s;
     max_rows = std::min(max_rows, a.rows.rows);
-    const AttnPlan p = plan_attention(a.rows.batch, a.cache.heads, a.cache.dim, a.cache.page_shift, a.group, max_rows, max_len, window, sinks, sms);
+    const AttnPlan p = plan_attention(a.rows.batch, a.cache.heads, a.cache.dim, a.cache.page_shift, a.group, a.rows.rows,
+                                      max_rows, max_len, window, sinks, sms);
     if (p.bytes) {
         if (!workspace || workspace_bytes < p.bytes) return refuse(TB_ERR_WORKSPACE, "workspace missing or too small");
         if (!aligned16(workspace)) return refuse(TB_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
@@ -401,9 +415,9 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     const bool bf16 = fmt == TB_FMT_BF16;
     cudaError_t e;
     if (a.cache.dim == 128)
-        e = bf16 ? run_attention<128, true>(a, p.nt, max_rows, sms, stream) : run_attention<128, false>(a, p.nt, max_rows, sms, stream);
+        e = bf16 ? run_attention<128, true>(a, p.nt, p.drawn, sms, stream) : run_attention<128, false>(a, p.nt, p.drawn, sms, stream);
     else
-        e = bf16 ? run_attention<64, true>(a, p.nt, max_rows, sms, stream) : run_attention<64, false>(a, p.nt, max_rows, sms, stream);
+        e = bf16 ? run_attention<64, true>(a, p.nt, p.drawn, sms, stream) : run_attention<64, false>(a, p.nt, p.drawn, sms, stream);
     return launched(e);
 }
 

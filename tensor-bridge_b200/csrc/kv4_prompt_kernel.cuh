@@ -75,7 +75,6 @@ struct PromptCfg {
     // Registers a thread: at launch, then by role.
     static constexpr int REGS = 96, REGS_SOFTMAX = 152, REGS_DECODE = 64, REGS_REST = 40;
     static_assert(256 * (REGS_SOFTMAX + REGS_DECODE) + 128 * REGS_REST <= kPromptThreads * REGS, "registers of the launch");
-    static constexpr int SLOT_FLOATS = kPromptRows * (D + 2);
 };
 
 // Low word of the descriptor of an N-major operand tile (V as [token][d]): 64
@@ -124,11 +123,18 @@ __device__ __forceinline__ PromptUnit prompt_rows(const Kv4Attn& a, int b, int h
     return u;
 }
 
-// Where the partial results of a unit's share lie.
+// Partial results lie by share, KV head and packed row of the whole call: all
+// o, then all m, then all l.  The number of a unit's first row among them.
+__device__ __forceinline__ size_t prompt_slot(const Kv4Attn& a, const PromptUnit& u, int split) {
+    return (static_cast<size_t>(split) * a.cache.heads + u.head) * a.rows.rows * a.group +
+           static_cast<size_t>(u.q.first) * a.group + u.row_base;
+}
 template <class C>
-__device__ __forceinline__ float* prompt_slot(const Kv4Attn& a, const PromptUnit& u, int split) {
-    const size_t unit = (static_cast<size_t>(u.b) * a.prompt_tiles + u.row_base / kPromptRows) * a.cache.heads + u.head;
-    return a.prompt_ws + (unit * a.prompt_splits + split) * C::SLOT_FLOATS;
+__device__ __forceinline__ float* prompt_m(const Kv4Attn& a) {
+    return a.prompt_ws + static_cast<size_t>(a.prompt_splits) * a.cache.heads * a.rows.rows * a.group * C::D;
+}
+__device__ __forceinline__ size_t prompt_m_to_l(const Kv4Attn& a) {
+    return static_cast<size_t>(a.prompt_splits) * a.cache.heads * a.rows.rows * a.group;
 }
 
 // Item number `item`: share (item % splits) of unit item / splits.  A unit is a
@@ -582,7 +588,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             // products have ended), D / 8 chunks of 16 bytes of a row at a time,
             // chunk x at x ^ (row & 7) of its panel, so that they leave in whole
             // lines: with a row a thread this took 5 us an item.
-            float* slot = prompt_slot<C>(a, u, u.split);
+            float* slot = a.prompt_ws + prompt_slot(a, u, u.split) * D;
             uint8_t* stage = q_tile + warp_row * 128;
             uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(u.head) * a.group * D +
                             8 * (lane % PromptQ<C>::LANES);
@@ -659,8 +665,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             PromptQ<C> q;
             if (item_next >= 0) prompt_q_load<C>(a, un, t * 128 + warp_row, q);
             if (row.valid && partial) {
-                slot[kPromptRows * D + t * 128 + r] = m;
-                slot[kPromptRows * (D + 1) + t * 128 + r] = l;
+                float* at = prompt_m<C>(a) + prompt_slot(a, u, u.split) + t * 128 + r;
+                at[0] = m;
+                at[prompt_m_to_l(a)] = l;
             } else if (row.valid && a.lse != nullptr) {
                 a.lse[static_cast<long long>(row.at) * a.q_heads + row.head] =
                     l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
@@ -961,30 +968,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
     grid_dep_wait();
 }
 
-// Joins the splits of the prompt kernel's units, in their order.  blockIdx.y
-// takes 256 / D of a unit's rows.
+// Joins the splits of the prompt kernel's rows, in their order: 256 / D packed
+// rows of KV head blockIdx.y to a CTA.
 template <class C, bool BF16>
 __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4Attn a) {
-    constexpr int D = C::D, LANES = D / 4;
-    const int per = a.cache.heads * a.prompt_tiles, b = blockIdx.x / per, tile = blockIdx.x % a.prompt_tiles;
-    const int quarter = threadIdx.x / 64, item = threadIdx.x % 64;
-    const int r = blockIdx.y * (64 / LANES) + item / LANES, d = 4 * (item % LANES);
-    const PromptUnit u = prompt_rows(a, b, (blockIdx.x - b * per) / a.prompt_tiles, tile);
-    if (!u.any || static_cast<int>(blockIdx.y) * (64 / LANES) >= u.row_count) return;
-    const bool valid = r < u.row_count;
-    const long long tiles = u.t1;
+    constexpr int D = C::D, LANES = D / 4, ROWS = 64 / LANES;
+    __shared__ int seq[ROWS];
+    const int row0 = blockIdx.x * ROWS;
+    if (a.rows.batch > 1) {  // one needs no search, a trip to memory less
+        if (threadIdx.x < ROWS) seq[threadIdx.x] = -1;
+        __syncthreads();
+        for (int b = threadIdx.x; b < a.rows.batch; b += blockDim.x) {
+            const int c0 = a.rows.cu[b], c1 = a.rows.cu[b + 1];
+            for (int i = 0; i < ROWS; ++i) {
+                const int at = (row0 + i) / a.group;
+                if (c0 <= at && at < c1) seq[i] = b;
+            }
+        }
+        __syncthreads();
+    }
+    const int quarter = threadIdx.x / 64, item = threadIdx.x % 64, d = 4 * (item % LANES);
+    const int b = a.rows.batch > 1 ? seq[item / LANES] : 0, row = row0 + item / LANES;
+    PromptUnit u;
+    int r = 0;  // row of the unit
+    u.any = false;
+    if (b >= 0 && row < a.rows.rows * a.group) {
+        const Kv4Seq q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
+        const int packed = row - q.first * a.group, tile = packed / kPromptRows;
+        r = packed - tile * kPromptRows;
+        u.any = packed >= 0 && packed < q.n * a.group && tile < a.prompt_tiles;
+        if (u.any) u = prompt_rows(a, b, blockIdx.y, tile);
+    }
+    if (!__syncthreads_or(u.any)) return;
     float top = kNoMax, l = 0.0f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (valid) {
+    if (u.any) {
+        const long long tiles = u.t1;
+        const float* ml = prompt_m<C>(a);
+        const size_t to_l = prompt_m_to_l(a);
 #pragma unroll 4
         for (int s = quarter; s < a.prompt_splits; s += 4) {
             if (tiles * s / a.prompt_splits == tiles * (s + 1) / a.prompt_splits) continue;  // no tiles, no result
-            const float* slot = prompt_slot<C>(a, u, s);
-            kv4_merge(top, l, v, slot[kPromptRows * D + r], slot[kPromptRows * (D + 1) + r],
-                      *reinterpret_cast<const float4*>(slot + r * D + d));
+            const size_t at = prompt_slot(a, u, s) + r;
+            kv4_merge(top, l, v, ml[at], ml[at + to_l], *reinterpret_cast<const float4*>(a.prompt_ws + at * D + d));
         }
     }
-    join_and_store<BF16, D>(a, valid, u.q.first, u.row_base + r, u.head, d, top, l, v);
+    join_and_store<BF16, D>(a, u.any, u.q.first, u.row_base + r, u.head, d, top, l, v);
 }
 
 }  // namespace tb
