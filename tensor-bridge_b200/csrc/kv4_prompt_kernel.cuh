@@ -124,10 +124,11 @@ __device__ __forceinline__ PromptUnit prompt_rows(const Kv4Attn& a, int b, int h
 }
 
 // Partial results lie by share, KV head and packed row of the whole call: all
-// o, then all m, then all l.  The number of a unit's first row among them.
-__device__ __forceinline__ size_t prompt_slot(const Kv4Attn& a, const PromptUnit& u, int split) {
-    return (static_cast<size_t>(split) * a.cache.heads + u.head) * a.rows.rows * a.group +
-           static_cast<size_t>(u.q.first) * a.group + u.row_base;
+// o, then all m, then all l.  The number of a unit's first row among them, which
+// the workspace (264 bytes and more to each) keeps far below 2^31; a 64-bit
+// address cost registers (a prompt of 4096 tokens 165 us for 162).
+__device__ __forceinline__ uint32_t prompt_slot(const Kv4Attn& a, const PromptUnit& u, int split) {
+    return static_cast<uint32_t>(((split * a.cache.heads + u.head) * a.rows.rows + u.q.first) * a.group + u.row_base);
 }
 template <class C>
 __device__ __forceinline__ float* prompt_m(const Kv4Attn& a) {
@@ -588,7 +589,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             // products have ended), D / 8 chunks of 16 bytes of a row at a time,
             // chunk x at x ^ (row & 7) of its panel, so that they leave in whole
             // lines: with a row a thread this took 5 us an item.
-            float* slot = a.prompt_ws + prompt_slot(a, u, u.split) * D;
+            const uint32_t slot = partial ? prompt_slot(a, u, u.split) : 0u;
             uint8_t* stage = q_tile + warp_row * 128;
             uint16_t* out = static_cast<uint16_t*>(a.out) + static_cast<long long>(u.head) * a.group * D +
                             8 * (lane % PromptQ<C>::LANES);
@@ -650,7 +651,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                         const int tr = t * 128 + warp_row + rr;
                         if (tr < u.row_count) {
                             if (partial)
-                                *reinterpret_cast<uint4*>(slot + tr * D + col + 4 * x) = v[k];
+                                *reinterpret_cast<uint4*>(a.prompt_ws + static_cast<size_t>(slot + tr) * D + col + 4 * x) = v[k];
                             else
                                 *reinterpret_cast<uint4*>(out + at * a.out_stride + head * D) = v[k];
                         }
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             PromptQ<C> q;
             if (item_next >= 0) prompt_q_load<C>(a, un, t * 128 + warp_row, q);
             if (row.valid && partial) {
-                float* at = prompt_m<C>(a) + prompt_slot(a, u, u.split) + t * 128 + r;
+                float* at = prompt_m<C>(a) + slot + t * 128 + r;
                 at[0] = m;
                 at[prompt_m_to_l(a)] = l;
             } else if (row.valid && a.lse != nullptr) {
@@ -1009,7 +1010,7 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4Attn a) {
 #pragma unroll 4
         for (int s = quarter; s < a.prompt_splits; s += 4) {
             if (tiles * s / a.prompt_splits == tiles * (s + 1) / a.prompt_splits) continue;  // no tiles, no result
-            const size_t at = prompt_slot(a, u, s) + r;
+            const size_t at = prompt_slot(a, u, s) + static_cast<uint32_t>(r);
             kv4_merge(top, l, v, ml[at], ml[at + to_l], *reinterpret_cast<const float4*>(a.prompt_ws + at * D + d));
         }
     }
