@@ -198,8 +198,9 @@ AttnPlan plan_attention(int batch, int heads, int dim, int page_shift, int group
         // with 1024).
         // Unlike sequences have about as many units as their rows fill tiles: 128
         // rows behind 32640 tokens and 31 single rows 594 us, 1032 without shares.
-        const long long tiles = p.drawn ? (static_cast<long long>(call_rows) * group + kPromptRows - 1) / kPromptRows
-                                        : static_cast<long long>(batch) * p.prompt_tiles;
+        // Rows of a padded batch count too: the partial results have their place.
+        long long tiles = (static_cast<long long>(call_rows) * group + kPromptRows - 1) / kPromptRows;
+        if (!p.drawn) tiles = std::max(tiles, static_cast<long long>(batch) * p.prompt_tiles);
         p.splits = static_cast<int>(std::max(1ll, std::min(sms / std::max(tiles * heads, 1ll), max_len / 512ll)));
         p.bytes += 16;  // the items' counter
         if (p.splits > 1)

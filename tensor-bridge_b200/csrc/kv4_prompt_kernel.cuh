@@ -124,9 +124,9 @@ __device__ __forceinline__ PromptUnit prompt_rows(const Kv4Attn& a, int b, int h
 }
 
 // Partial results lie by share, KV head and packed row of the whole call: all
-// o, then all m, then all l.  The number of a unit's first row among them, which
-// the workspace (264 bytes and more to each) keeps far below 2^31; a 64-bit
-// address cost registers (a prompt of 4096 tokens 165 us for 162).
+// o, then all m, then all l.  The number of a unit's first row among them: tiles
+// of 256 rows of the call * heads * splits are no more than the SMs, so it is
+// small; a 64-bit address cost registers (a prompt of 4096 tokens 165 us for 162).
 __device__ __forceinline__ uint32_t prompt_slot(const Kv4Attn& a, const PromptUnit& u, int split) {
     return static_cast<uint32_t>(((split * a.cache.heads + u.head) * a.rows.rows + u.q.first) * a.group + u.row_base);
 }

@@ -802,6 +802,14 @@ def test_workspace_is_asked_for(tb, cuda):
         assert e.value.status == tb.Status[st]
 
 
+def test_workspace_of_a_padded_batch(tb, cuda):
+    """Rows of nobody, far more than the others, do not swell the workspace."""
+    bt = Batch(tb, cuda, [1500], [20], page=16, heads=2, dim=64, seed=61, pad=9000)
+    bt.fill_fast()
+    assert tb.kv4_attention_workspace(bt.cache, bt.rows, 8, 20, LONG) < 64 * 2 ** 20
+    bt.run(8)
+
+
 @pytest.mark.parametrize("typ", ["f16", "bf16"])
 def test_prompt_then_steps(tb, cuda, typ):
     """The operators together, as a generation runs them: a prompt's rows are
