@@ -326,18 +326,20 @@ typedef struct tb_kv4_cache {
  * n = cu_rows[b+1] - cu_rows[b]: a sequence's rows are its last n tokens, and
  * seq_lens counts them.  Token t is in page block_table[b][t / page_size].
  * The three arrays are on the device and read when the kernels run, so a
- * captured call follows their contents.  cu_rows does not decrease; rows from
- * cu_rows[batch] to `rows` belong to nobody (a padded batch): they are not
- * read and what would be written to them stays as it was.  Table entries
- * behind a sequence's last page are not read.
+ * captured call follows their contents.  cu_rows does not decrease and stays
+ * within 0 and `rows`; rows from cu_rows[batch] to `rows` belong to nobody (a
+ * padded batch): they are not read and what would be written to them stays as
+ * it was.  Table entries behind a sequence's last page are not read.
  * Pages that a window hides from all of a sequence's rows may be gone: their
  * entries may hold any number (another sequence's page, -1).
  * Contents that the host cannot check are checked on the device: a row whose
  * token number is negative or whose page is not in [0, num_pages) or not in
  * the table is left out (not written, not read back, not seen by attention;
- * an attention row of negative token number sees nothing), rows outside `rows`
- * are not touched, and bit 1 of tb_device_error's word is set (not by
- * attention for negative token numbers alone). */
+ * an attention row of negative token number sees nothing), rows that cu_rows
+ * places outside `rows` are not touched (the same sequence's others keep their
+ * token numbers), and bit 1 of tb_device_error's word is set: for any cu_rows
+ * that leaves `rows` or decreases too, but not by attention for negative token
+ * numbers alone. */
 typedef struct tb_kv4_rows {
     const int32_t* cu_rows;     /* device [batch + 1] */
     const int32_t* seq_lens;    /* device [batch] */

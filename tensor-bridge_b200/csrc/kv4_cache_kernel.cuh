@@ -62,6 +62,7 @@ __device__ __forceinline__ void kv4_find_rows(const Kv4Copy& a, int row0, Kv4Pla
         const int c0 = a.rows.cu[b], c1 = a.rows.cu[b + 1];
         for (int i = 0; i < ROWS; ++i)
             if (c0 <= row0 + i && row0 + i < c1) s.seq[i] = b;
+        if (row0 == 0 && blockIdx.y == 0 && (c0 < 0 || c1 < c0 || c1 > a.rows.rows)) atomicOr(&g_tb_device_error, kErrPage);
     }
     __syncthreads();
     if (threadIdx.x < ROWS) {
@@ -70,7 +71,7 @@ __device__ __forceinline__ void kv4_find_rows(const Kv4Copy& a, int row0, Kv4Pla
         int place = 0;
         if (b >= 0 && row0 + i < a.rows.rows) {
             const int shift = a.cache.page_shift;
-            const Kv4Seq q = kv4_seq(a.rows, shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
+            const Kv4Seq q = kv4_rows_seq(a.rows, shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
             const int pos = q.pos0 + (row0 + i - q.first);
             const int slot = pos >> shift;
             bool ok = pos >= 0 && kv4_slot_ok(a.rows, slot);

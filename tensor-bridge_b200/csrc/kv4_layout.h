@@ -57,8 +57,10 @@ struct Kv4Seq {
     int len;      // tokens of the sequence that the table has pages for
     int pos0;     // position of row `first`; negative where n > length
     bool bad;     // the length is negative or passes the table
+    bool cut;     // cu decreases, or some of the rows lie outside the caller's
 };
 
+// The rows as clamped, the last of them the sequence's last token.
 TB_KV4_HD Kv4Seq kv4_seq(const Kv4Rows& r, int page_shift, int cu0, int cu1, int len) {
     Kv4Seq s;
     s.first = cu0 < 0 ? 0 : cu0 > r.rows ? r.rows : cu0;
@@ -68,6 +70,22 @@ TB_KV4_HD Kv4Seq kv4_seq(const Kv4Rows& r, int page_shift, int cu0, int cu1, int
     s.bad = len < 0 || len > room;
     s.len = len < 0 ? 0 : len > room ? static_cast<int>(room) : len;
     s.pos0 = (len < 0 ? 0 : len) - s.n;
+    s.cut = cu0 < 0 || cu1 < cu0 || cu1 > r.rows;
+    return s;
+}
+
+// The same with each row at its own token: rows behind the caller's arrays are
+// the sequence's last tokens, those inside come before them.  The position of
+// row `first` is len - (cu1 - first); where that is below -2^31 + 4096 (then all
+// rows inside are before the sequence) it is held there, so that what the
+// kernels add and subtract stays in 32 bits.
+TB_KV4_HD Kv4Seq kv4_rows_seq(const Kv4Rows& r, int page_shift, int cu0, int cu1, int len) {
+    Kv4Seq s = kv4_seq(r, page_shift, cu0, cu1, len);
+    if (s.n > 0) {
+        const long long pos0 = (len < 0 ? 0ll : len) - (static_cast<long long>(cu1) - s.first);
+        constexpr int kLeast = -0x7FFFFFFF - 1 + 4096;
+        s.pos0 = pos0 < kLeast ? kLeast : static_cast<int>(pos0);
+    }
     return s;
 }
 

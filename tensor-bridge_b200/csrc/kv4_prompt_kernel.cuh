@@ -110,7 +110,7 @@ __device__ __forceinline__ PromptUnit prompt_rows(const Kv4Attn& a, int b, int h
     u.b = b;
     u.head = head;
     u.split = 0;
-    u.q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[u.b], a.rows.cu[u.b + 1], a.rows.lens[u.b]);
+    u.q = kv4_rows_seq(a.rows, a.cache.page_shift, a.rows.cu[u.b], a.rows.cu[u.b + 1], a.rows.lens[u.b]);
     u.row_base = tile * kPromptRows;
     u.row_count = min(kPromptRows, u.q.n * a.group - u.row_base);
     u.t0 = u.t1 = 0;
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
         seqs = 0;
         for (int b0 = 0; b0 < a.rows.batch; b0 += kPromptThreads) {
             const int b = b0 + tid;
-            const bool here = b < a.rows.batch && prompt_takes(a, kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[b],
+            const bool here = b < a.rows.batch && prompt_takes(a, kv4_rows_seq(a.rows, a.cache.page_shift, a.rows.cu[b],
                                                                           a.rows.cu[b + 1], a.rows.lens[b]));
             const uint32_t some = __ballot_sync(0xFFFFFFFFu, here);
             if (lane == 0) warp_sums[warp] = __popc(some);
@@ -994,7 +994,7 @@ __global__ void __launch_bounds__(256) k_kv4_prompt_join(const Kv4Attn a) {
     int r = 0;  // row of the unit
     u.any = false;
     if (b >= 0 && row < a.rows.rows * a.group) {
-        const Kv4Seq q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
+        const Kv4Seq q = kv4_rows_seq(a.rows, a.cache.page_shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
         const int packed = row - q.first * a.group, tile = packed / kPromptRows;
         r = packed - tile * kPromptRows;
         u.any = packed >= 0 && packed < q.n * a.group && tile < a.prompt_tiles;

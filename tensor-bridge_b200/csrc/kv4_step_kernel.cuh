@@ -222,15 +222,17 @@ struct StepSeq {
 template <class C>
 __device__ __forceinline__ StepSeq step_seq(const Kv4Attn& a, int b) {
     StepSeq s;
-    s.q = kv4_seq(a.rows, a.cache.page_shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
+    s.q = kv4_rows_seq(a.rows, a.cache.page_shift, a.rows.cu[b], a.rows.cu[b + 1], a.rows.lens[b]);
     s.span = kv4_span(s.q.pos0, s.q.pos0 + s.q.n - 1, s.q.len, a.window, a.sinks, step_gran(a.cache.page_shift, C::GRAN_MOST));
     const long long rows = static_cast<long long>(s.q.n) * a.group;
     s.chunks = rows > 0 && rows <= a.step_rows ? kv4_span_chunks(s.span) : 0;
     return s;
 }
 
-// Reports a sequence that neither kernel takes: more rows than max_rows said.
+// Reports a sequence with rows outside the caller's, and one that neither
+// kernel takes: more rows than max_rows said.
 __device__ __forceinline__ void step_report(const Kv4Attn& a, const StepSeq& s) {
+    if (s.q.cut) atomicOr(&g_tb_device_error, kErrPage);
     if (a.prompt_tiles == 0 && static_cast<long long>(s.q.n) * a.group > a.step_rows)
         atomicOr(&g_tb_device_error, kErrRows);
 }

