@@ -385,6 +385,8 @@ tb_status tb_kv4_read(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_for
  *   out = sum_j e^{s_j} v_j / sum_j e^{s_j},   s_j = softmax_scale * q . k_j
  *   lse = ln sum_j e^{s_j}            (device [rows x q_heads] FP32, or NULL)
  * A row that sees nothing, or only scores of -inf, has out = 0, lse = -inf.
+ * Sums and lse are FP32; the weights e^{s_j} are rounded to FP16 for the first
+ * product, each by 2^-11 of itself or 2^-31 of the row's largest.
  * max_rows is at least the rows of any sequence (with fewer, bit 2 of
  * tb_device_error's word is set and rows may be missing); max_len is the
  * longest sequence, and only steers how the work is split.  The result does

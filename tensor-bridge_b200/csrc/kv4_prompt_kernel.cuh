@@ -24,10 +24,10 @@
 // the converter second value first; Q is stored in the same order, and the
 // output's columns are swapped back when they are read.
 //
-// The maximum m of a row is moved only when a score passes it by 2^8 (2^15 in
-// the second half of a tile), so the usual tile takes one pass: exponentials
-// with the old m, the largest score found along the way, and a second pass
-// (with O scaled in TMEM) only if it passed.  S_t of a tile is issued behind
+// The maximum m of a row is moved only when a score passes it by 2^15, to 2^7
+// below that score, so the usual tile takes one pass: exponentials with the old
+// m, the largest score found along the way, and a second pass (with O scaled in
+// TMEM) only if it passed.  S_t of a tile is issued behind
 // P_t V of the tile before, so a thread that sees S_t finds O_t at rest.
 //
 // What bounds it: a row tile and token tile (128 x 128, D = 128) needs 1024
@@ -35,7 +35,8 @@
 // 2300: S_t waits for P_t V and P_t for S_t, so that the two tiles' phases
 // overlap only in part, and what the softmax warps issue beside the exponentials
 // (scale, maximum, sum, packing) shares its slots with the decoding warps.
-// P below 2^8 or 2^15 is rounded to FP16 (2^-11), l is summed in FP32.
+// P below 2^15 is rounded to FP16 as in the step kernel (m is a whole number here,
+// so P's largest may lie at 2^6), l is summed in FP32.
 // Measured, 32 heads of 128, 8 KV heads: a prompt of 4096 tokens 162 us (848
 // TFLOP/s, 0.52 of a bf16 GEMM), 2048 rows behind 14336 tokens 544 us (950
 // TFLOP/s); ends of items cost ~14000 cycles each, hence whole rounds of large
@@ -517,14 +518,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
                     if (half == 1 || j > u.t0)
                         top = open ? prompt_pass<false>(s_half, f, m, m0, m1, p, &sum)
                                    : prompt_pass<true>(s_half, f, m, m0, m1, p, &sum);
-                    // The first half keeps P below 2^8, the second below 2^15,
-                    // since moving m there waits for the first half's P V.
-                    const bool move = top > (half == 0 ? 8.0f : 15.0f);
+                    const bool move = top > kPMost;
                     if (__any_sync(0xFFFFFFFFu, move)) {
                         // The row's largest score, found anew: s f - m has lost
                         // it where m was kNoMax.  m stays a whole number, so
                         // that what is scaled by its steps is not rounded.
-                        const float y = ceilf(prompt_top(s_half, f, m0, m1));
+                        const float y = ceilf(prompt_top(s_half, f, m0, m1)) - kPSet;
                         const float m_new = move ? fmaxf(m, y) : m;  // the warp's other rows go through the same values again
                         const float step = m_new - m;
                         const float scale = step < 126.0f ? exp2i(-static_cast<int>(step)) : 0.0f;

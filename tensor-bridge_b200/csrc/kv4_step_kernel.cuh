@@ -21,10 +21,15 @@
 //     tokens are interleaved before they are converted (two operations for
 //     eight values), not the FP16 values after (four).
 //   - P^T's fragment is S^T's, transposed in 8 x 8 blocks: movmatrix.
-//   - the maximum is moved only when a score passes it by 2^8: P stays below
-//     2^8, far inside FP16, and the reductions over lanes are rare.
-// P is rounded to FP16 (2^-11), finer than either output type is to a sum's
-// terms; l is summed from the FP32 values.
+//   - the maximum is moved only when a score passes it by 2^15, and is then set
+//     2^7 below the largest score: P stays below 2^15, inside FP16, and the
+//     reductions over lanes are rare.
+// P is rounded to FP16: by 2^-11 of itself down to 2^-21 of the row's largest
+// (P's largest is 2^7 at least), below that, where FP16 is subnormal, by up to
+// 2^-32 of the largest.  So where a row's weight lies on a few tokens of no value
+// the sum of the others is good to 1% while they are above 2^-25; with P at 1 at
+// most it was off by 13% at 2^-22 and all of it was lost at 2^-26.
+// l is summed from the FP32 values.
 //
 // BF16 queries are scaled per row by a power of two to at most 2^15 and taken
 // as FP16: exact for values within 2^-28 of the row's largest, and off by at
@@ -79,6 +84,10 @@ constexpr int kStepChunk = 32;     // tokens of a warp's share of a tile
 // A row's maximum before it has seen a score: finite, so that differences are
 // ordinary numbers; every score passes it.
 constexpr float kNoMax = -1e38f;
+// In log2 units: a score that passes the row's m by more than kPMost moves it, to
+// kPSet below the largest score.  P is then at most 2^7, far from the 2^-14 where
+// FP16 loses bits, and other scores may be 2^8 times larger until m moves again.
+constexpr float kPMost = 15.0f, kPSet = 7.0f;
 constexpr int kStepRowsMost = 32;  // packed rows of a (sequence, KV head)
 
 // NT tiles of eight rows.  Eight computing warps, and twelve for two tiles,
@@ -664,14 +673,14 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
                             }
                     }
             }
-            // In log2 units a score is s f - m; a row whose largest passes 2^8 moves its m.
+            // In log2 units a score is s f - m; a row whose largest passes kPMost moves its m.
             bool past = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     past |= fmaf(fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2])),
-                                 sf[nt][e], -m[nt][e]) > 8.0f;
+                                 sf[nt][e], -m[nt][e]) > kPMost;
             if (__builtin_expect(__any_sync(0xFFFFFFFFu, past), 0)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -680,7 +689,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
                         float y = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xFFFFFFFFu, y, d));
-                        y = fmaxf(y * sf[nt][e], m[nt][e]);
+                        y = fmaxf(fmaf(y, sf[nt][e], -kPSet), m[nt][e]);
                         const float r = ex2(m[nt][e] - y);
                         m[nt][e] = y;
                         l[nt][e] *= r;
