@@ -300,7 +300,7 @@ __device__ __forceinline__ void prompt_q_store(const Kv4Attn& a, const PromptQ<C
     for (int x = 0; x < Q::N; ++x) {
         const int rr = r0 + x * Q::AT_ONCE + lane / Q::LANES;
         uint32_t w[4] = {q.v[x].x, q.v[x].y, q.v[x].z, q.v[x].w};
-        float f = fmaxf(fabsf(a.scale_log2), 1e-37f);
+        float f = fabsf(a.scale_log2);
         if constexpr (BF16) {
             uint32_t e = 0;
 #pragma unroll
@@ -309,7 +309,7 @@ __device__ __forceinline__ void prompt_q_store(const Kv4Attn& a, const PromptQ<C
             for (int d = 1; d < Q::LANES; d <<= 1) e = max(e, __shfl_xor_sync(0xFFFFFFFFu, e, d));
             const int kk = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = kk > 120 ? 120 : kk, k2 = kk - k1;
             const float up = exp2i(k1), up2 = exp2i(k2);
-            f = fmaxf((f * exp2i(-k1)) * exp2i(-k2), 1e-37f);
+            f = (f * exp2i(-k1)) * exp2i(-k2);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 w[j] = pack_half2(__uint_as_float(w[j] & 0xFFFF0000u) * up * up2, __uint_as_float(w[j] << 16) * up * up2);
@@ -317,7 +317,7 @@ __device__ __forceinline__ void prompt_q_store(const Kv4Attn& a, const PromptQ<C
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = prmt(w[j], 0u, 0x1032u);
         }
-        if (k == 0) scale[rr] = f;
+        if (k == 0) scale[rr] = kv4_row_factor(f);
         *reinterpret_cast<uint4*>(tile + (k / 8) * C::PANEL + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) =
             make_uint4(w[0] ^ sign, w[1] ^ sign, w[2] ^ sign, w[3] ^ sign);
     }

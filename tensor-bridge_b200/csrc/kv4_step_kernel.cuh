@@ -200,6 +200,11 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// A row's factor from products to scores, last of all steps: not zero, which
+// would make NaN of a hidden score's -inf, and not infinite, which would of a
+// product that is zero.
+__device__ __forceinline__ float kv4_row_factor(float scale) { return fminf(fmaxf(scale, 1e-37f), 3e38f); }
+
 // log2 of the tokens of a chunk, in which sequences are split: a page's, but 32
 // at least (a warp's share) and `most` at most (it divides a tile).
 TB_KV4_HD int step_gran(int page_shift, int most) {
@@ -528,8 +533,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
         for (int r = warp; r < ROWS; r += WARPS) {
             uint2 v = make_uint2(0u, 0u);
             // The factor is taken positive, its sign into q: the largest product
-            // is the largest score.  Not zero, which would make NaN of -inf.
-            float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);
+            // is the largest score.
+            float scale = fabsf(a.scale_log2);
             const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
             if (r < row_count) {
                 const int i = r / a.group;
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
                     e = __reduce_max_sync(0xFFFFFFFFu, e);
                     const int k = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = k > 120 ? 120 : k, k2 = k - k1;
                     const float up = exp2i(k1), up2 = exp2i(k2);
-                    scale = fmaxf((scale * exp2i(-k1)) * exp2i(-k2), 1e-37f);
+                    scale = (scale * exp2i(-k1)) * exp2i(-k2);
                     v.x = pack_half2(__uint_as_float(v.x << 16) * up * up2, __uint_as_float(v.x & 0xFFFF0000u) * up * up2);
                     v.y = pack_half2(__uint_as_float(v.y << 16) * up * up2, __uint_as_float(v.y & 0xFFFF0000u) * up * up2);
                 }
@@ -556,7 +561,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
                 qfrag[((r / 8) * KS + ks) * 32 + (r % 8) * 4 + cc] =
                     make_uint2(prmt(v.x, 0u, 0x1032u), prmt(v.y, 0u, 0x1032u));
             }
-            if (lane == 0) sm_scale[r] = scale;
+            if (lane == 0) sm_scale[r] = kv4_row_factor(scale);
         }
         named_bar_sync(1, 32 * WARPS);
 
