@@ -307,7 +307,7 @@ __device__ __forceinline__ void prompt_q_store(const Kv4Attn& a, const PromptQ<C
             for (int j = 0; j < 4; ++j) e = max(e, max((w[j] >> 7) & 0xFFu, (w[j] >> 23) & 0xFFu));
 #pragma unroll
             for (int d = 1; d < Q::LANES; d <<= 1) e = max(e, __shfl_xor_sync(0xFFFFFFFFu, e, d));
-            const int kk = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = kk > 120 ? 120 : kk, k2 = kk - k1;
+            const int kk = e == 255u ? -113 : 141 - static_cast<int>(e), k1 = kk > 120 ? 120 : kk, k2 = kk - k1;
             const float up = exp2i(k1), up2 = exp2i(k2);
             f = (f * exp2i(-k1)) * exp2i(-k2);
 #pragma unroll

@@ -543,11 +543,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) k_kv4_step(const Kv4Attn 
                 if (lane < D / 4) v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + at);
                 if constexpr (BF16) {
                     // Exponent of the row's largest value -> 2^k that brings it to [2^14, 2^15),
-                    // in two factors (k passes 127 for the smallest rows); not for infinity and NaN.
+                    // in two factors (k passes 127 for the smallest rows).  Where it is infinity or
+                    // NaN all scores are, whatever the others are: they only have to stay finite.
                     uint32_t e = max(max((v.x >> 7) & 0xFFu, (v.x >> 23) & 0xFFu),
                                      max((v.y >> 7) & 0xFFu, (v.y >> 23) & 0xFFu));
                     e = __reduce_max_sync(0xFFFFFFFFu, e);
-                    const int k = e == 255u ? 0 : 141 - static_cast<int>(e), k1 = k > 120 ? 120 : k, k2 = k - k1;
+                    const int k = e == 255u ? -113 : 141 - static_cast<int>(e), k1 = k > 120 ? 120 : k, k2 = k - k1;
                     const float up = exp2i(k1), up2 = exp2i(k2);
                     scale = (scale * exp2i(-k1)) * exp2i(-k2);
                     v.x = pack_half2(__uint_as_float(v.x << 16) * up * up2, __uint_as_float(v.x & 0xFFFF0000u) * up * up2);

@@ -1,6 +1,7 @@
 """Attention over the FP4 cache where the factor of the scores or the queries
 lie at the ends of their ranges."""
-import numpy as np
+import math
+
 import pytest
 
 from test_kv4_gpu import LONG, Batch, error_word  # noqa: F401 (error_word: a fixture)
@@ -35,3 +36,25 @@ def test_large_factor_of_zero_products(tb, cuda, n, max_len):
     q *= 2.0 ** 120
     out, lse = bt.attend(q, 4, 2.0 ** 40, max_len=max_len)
     bt.check(out, lse, q, 4, 2.0 ** 40)
+
+
+@pytest.mark.parametrize("max_len", [None, LONG])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_infinite_query_beside_large_ones(tb, cuda, n, max_len):
+    """BF16 rows that hold -inf where all keys are positive, beside values far
+    outside FP16: all their scores are -inf.  The other rows stay as they are."""
+    bt = Batch(tb, cuda, [n + 60, n + 300], [n, n], page=16, heads=1, dim=64, typ="bf16", seed=n)
+    bt.fill_fast()
+    for page in range(bt.host.pages):
+        at = bt.host.data[page, :bt.host.codes].reshape(16, 32)
+        at[:, 0] = 0x20 | at[:, 0] & 7  # token's first value 1.0, the second not negative
+    bt.upload()
+    q, _ = bt.queries(2)
+    clean, clean_lse = bt.attend(q, 2, 0.1, max_len=max_len)
+    q[0, 0], q[0, 1:64] = -math.inf, 3e38
+    q[-1, 64], q[-1, 65] = -math.inf, -1e10
+    out, lse = bt.attend(q, 2, 0.1, max_len=max_len)
+    for row, head in ((0, 0), (bt.total - 1, 1)):
+        assert bool((out[row, 64 * head:64 * head + 64] == 0).all()) and lse[row, head].item() == -math.inf
+        clean[row, 64 * head:64 * head + 64], clean_lse[row, head] = 0, -math.inf
+    assert cuda.equal(out, clean) and cuda.equal(lse, clean_lse)
