@@ -344,9 +344,9 @@ typedef struct tb_kv4_rows {
     const int32_t* cu_rows;     /* device [batch + 1] */
     const int32_t* seq_lens;    /* device [batch] */
     const int32_t* block_table; /* device [batch x table_width] */
-    int batch;
+    int batch;                  /* < 2^31 - 4096 */
     int table_width;            /* table_width * page_size < 2^31 - 4096 */
-    int rows;                   /* rows that the K, V, q and out arrays hold */
+    int rows;                   /* rows that the K, V, q and out arrays hold; < 2^31 - 4096 */
 } tb_kv4_rows;
 
 /* Bytes of a page: page_size * kv_heads * head_dim * 9 / 8. */

@@ -55,6 +55,9 @@ tb_status check_cache(const tb_kv4_cache* c, Kv4Cache* out) {
 tb_status check_rows(const tb_kv4_rows* r, int page_shift, Kv4Rows* out) {
     if (!r) return refuse(TB_ERR_INVALID_ARGUMENT, "rows is NULL");
     if (r->batch < 0 || r->rows < 0 || r->table_width < 0) return refuse(TB_ERR_SHAPE, "negative batch, rows or table_width");
+    // Kernels step over rows and sequences in 32 bits, by less than 4096 at a time.
+    if (r->batch > 0x7FFFFFFF - 4096 || r->rows > 0x7FFFFFFF - 4096)
+        return refuse(TB_ERR_SHAPE, "batch and rows must not pass 2^31 - 4097");
     if ((static_cast<long long>(r->table_width) << page_shift) > 0x7FFFFFFFll - 4096)
         return refuse(TB_ERR_SHAPE, "table_width * page_size must stay below 2^31 - 4096");
     if (r->batch && r->rows && (!r->cu_rows || !r->seq_lens || (!r->block_table && r->table_width)))
