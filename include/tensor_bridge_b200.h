@@ -379,7 +379,8 @@ tb_status tb_kv4_read(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_for
  * [rows x q_heads x head_dim] in fmt (F16 or BF16), 16-byte aligned, q_stride
  * and out_stride elements from row to row (0: dense; a multiple of 8); they
  * may be the same array only if they are the same rows exactly.  Query head h
- * reads KV head h / (q_heads / kv_heads).  The row of token number p sees
+ * reads KV head h / (q_heads / kv_heads); rows * q_heads < 2^30 and
+ * q_heads / kv_heads * head_dim < 2^31.  The row of token number p sees
  * token j if j <= p and (window == 0 or j > p - window or j < sinks); its own
  * token is in the cache (tb_kv4_append comes first).  Over the tokens seen,
  *   out = sum_j e^{s_j} v_j / sum_j e^{s_j},   s_j = softmax_scale * q . k_j

@@ -305,6 +305,9 @@ tb_status check_heads(const tb_kv4_cache* c, int q_heads, int max_rows, int max_
     if (c->head_dim != 64 && c->head_dim != 128)
         return refuse(TB_ERR_SHAPE, "attention needs a head_dim of 64 or 128");
     if (q_heads < 1 || q_heads % c->kv_heads) return refuse(TB_ERR_SHAPE, "q_heads must be a multiple of kv_heads");
+    // A query's place within its KV head's group is a 32-bit number of elements.
+    if (static_cast<long long>(q_heads / c->kv_heads) * c->head_dim > 0x7FFFFFFFll)
+        return refuse(TB_ERR_SHAPE, "q_heads / kv_heads * head_dim must stay below 2^31");
     if (max_rows < 0 || max_len < 0) return refuse(TB_ERR_SHAPE, "negative max_rows or max_len");
     return TB_OK;
 }

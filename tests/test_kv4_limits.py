@@ -14,3 +14,12 @@ def test_rows_and_batches_near_two_to_31(tb, f, size):
     assert f(tb, cache(tb), rows(tb, n=size)) == S.SHAPE
     assert f(tb, cache(tb), rows(tb, batch=size)) == S.SHAPE
     assert "4097" in tb.lib().tb_last_error().decode()
+
+
+def test_groups_of_heads_that_pass_two_to_31_elements(tb):
+    S = tb.Status
+    for dim, heads in ((64, 2 ** 25), (128, 2 ** 24), (128, 2 ** 29)):
+        c, r = cache(tb, heads=1, dim=dim), rows(tb, n=1)
+        assert attention(tb, c, r, heads=heads) == S.SHAPE
+        assert "q_heads / kv_heads" in tb.lib().tb_last_error().decode()
+        assert tb.kv4_attention_workspace(c, r, heads, 1, 1000) == 0
