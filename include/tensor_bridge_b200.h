@@ -385,6 +385,7 @@ tb_status tb_kv4_read(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_for
  * token is in the cache (tb_kv4_append comes first).  Over the tokens seen,
  *   out = sum_j e^{s_j} v_j / sum_j e^{s_j},   s_j = softmax_scale * q . k_j
  *   lse = ln sum_j e^{s_j}            (device [rows x q_heads] FP32, or NULL)
+ * with softmax_scale and softmax_scale * k_scale * log2(e) finite in FP32.
  * A row that sees nothing, or only scores of -inf, has out = 0, lse = -inf.
  * Sums and lse are FP32; the weights e^{s_j} are rounded to FP16 for the first
  * product, each by 2^-11 of itself or 2^-31 of the row's largest.

@@ -379,6 +379,9 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
         return refuse(TB_ERR_SHAPE, "rows * q_heads must stay below 2^30");
     if (window < 0 || sinks < 0) return refuse(TB_ERR_INVALID_ARGUMENT, "window and sinks must not be negative");
     if (!std::isfinite(softmax_scale)) return refuse(TB_ERR_INVALID_ARGUMENT, "softmax_scale must be finite");
+    a.scale_log2 = softmax_scale * a.cache.k_scale * 1.4426950408889634f;
+    if (!std::isfinite(a.scale_log2))
+        return refuse(TB_ERR_INVALID_ARGUMENT, "softmax_scale * k_scale * log2(e) must be an FP32 number");
     const long long width = static_cast<long long>(q_heads) * a.cache.dim;
     s = check_stride(&q_stride, width);
     if (s == TB_OK) s = check_stride(&out_stride, width);
@@ -393,7 +396,6 @@ tb_status tb_kv4_attention(const tb_kv4_cache* cache, const tb_kv4_rows* rows, t
     a.out_stride = out_stride;
     a.q_heads = q_heads;
     a.group = q_heads / a.cache.heads;
-    a.scale_log2 = softmax_scale * a.cache.k_scale * 1.4426950408889634f;
     a.window = window;
     a.sinks = sinks;
     int sms = 0;

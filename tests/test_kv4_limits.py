@@ -23,3 +23,11 @@ def test_groups_of_heads_that_pass_two_to_31_elements(tb):
         assert attention(tb, c, r, heads=heads) == S.SHAPE
         assert "q_heads / kv_heads" in tb.lib().tb_last_error().decode()
         assert tb.kv4_attention_workspace(c, r, heads, 1, 1000) == 0
+
+
+def test_factors_that_pass_fp32(tb):
+    """Each scale is an FP32 number, their product is not."""
+    S = tb.Status
+    for ks, scale in ((2.0 ** 100, 2.0 ** 30), (2.0 ** 100, -2.0 ** 30), (2.0 ** 64, 2.0 ** 64), (2.0 ** 60, 2.0 ** 67 * 1.9)):
+        assert attention(tb, cache(tb, ks=ks), rows(tb), scale=scale) == S.INVALID_ARGUMENT
+        assert "softmax_scale * k_scale" in tb.lib().tb_last_error().decode()
