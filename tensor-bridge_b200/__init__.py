@@ -71,28 +71,64 @@ def stored_bytes(fmt: Format, n: int) -> int:
     return (n * num + den - 1) // den
 
 
+def _pages_ptr(data, num_pages: int, page_bytes: int, page_stride: int):
+    """Address of a cache's pages; a tensor has to hold them where the cache
+    looks: dense, or with its first dimension page_stride bytes apart."""
+    if hasattr(data, "is_contiguous") and num_pages > 0:
+        size, stride = data.element_size(), page_stride or page_bytes
+        if data.is_contiguous():
+            if data.numel() * size < (num_pages - 1) * stride + page_bytes:
+                raise ValueError(f"data has {data.numel() * size} bytes, fewer than {num_pages} pages of {page_bytes}, "
+                                 f"{stride} apart")
+        elif not (data.shape[0] >= num_pages and data.stride(0) * size == stride and data[0].is_contiguous()
+                  and data[0].numel() * size >= page_bytes):
+            raise ValueError(f"data must be dense, or pages of {page_bytes} dense bytes, {stride} apart")
+    return _ptr(data)
+
+
+def _int32_ptr(x, name: str, least: int):
+    """Address of an index array; a tensor has to be dense int32 and hold what
+    is read of it."""
+    if hasattr(x, "is_contiguous"):
+        if str(x.dtype) != "torch.int32":
+            raise ValueError(f"{name} must be int32, not {x.dtype}")
+        if not x.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if x.numel() < least:
+            raise ValueError(f"{name} has {x.numel()} entries, fewer than {least}")
+    return _ptr(x)
+
+
 class KV4Cache(ctypes.Structure):
     """tb_kv4_cache: a paged key/value cache in block-scaled FP4.  `data` is a
-    torch tensor (kept alive by this object) or a device address."""
+    torch tensor (kept alive by this object) or a device address.  A tensor
+    that does not hold the pages is refused with a ValueError."""
     _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_size_t), ("num_pages", ctypes.c_int),
                 ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
                 ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
 
     def __init__(self, data, num_pages: int, page_size: int, kv_heads: int, head_dim: int, k_scale: float = 1.0,
                  v_scale: float = 1.0, page_stride: int = 0):
-        super().__init__(_ptr(data), page_stride, num_pages, page_size, kv_heads, head_dim, k_scale, v_scale)
+        at = _pages_ptr(data, num_pages, page_size * kv_heads * head_dim * 9 // 8, page_stride)
+        super().__init__(at, page_stride, num_pages, page_size, kv_heads, head_dim, k_scale, v_scale)
         self._keep = data
 
 
 class KV4Rows(ctypes.Structure):
     """tb_kv4_rows: which sequences a call's rows belong to and where their
     tokens are.  The three index arrays are int32 torch tensors (kept alive by
-    this object) or device addresses."""
+    this object) or device addresses.  A tensor of another type (torch.cumsum
+    makes int64 of int32), not contiguous or too short is refused with a
+    ValueError."""
     _fields_ = [("cu_rows", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
                 ("batch", ctypes.c_int), ("table_width", ctypes.c_int), ("rows", ctypes.c_int)]
 
     def __init__(self, cu_rows, seq_lens, block_table, batch: int, table_width: int, rows: int):
-        super().__init__(_ptr(cu_rows), _ptr(seq_lens), _ptr(block_table), batch, table_width, rows)
+        used = batch > 0 and rows > 0
+        super().__init__(_int32_ptr(cu_rows, "cu_rows", batch + 1 if used else 0),
+                         _int32_ptr(seq_lens, "seq_lens", batch if used else 0),
+                         _int32_ptr(block_table, "block_table", batch * table_width if used else 0),
+                         batch, table_width, rows)
         self._keep = (cu_rows, seq_lens, block_table)
 
 
