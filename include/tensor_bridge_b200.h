@@ -390,8 +390,9 @@ tb_status tb_kv4_read(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_for
  * Sums and lse are FP32; the weights e^{s_j} are rounded to FP16 for the first
  * product, each by 2^-11 of itself or 2^-31 of the row's largest.
  * max_rows is at least the rows of any sequence (with fewer, bit 2 of
- * tb_device_error's word is set and rows may be missing); max_len is the
- * longest sequence, and only steers how the work is split.  The result does
+ * tb_device_error's word is set and rows may be missing; 0 says that there are
+ * none: the call does nothing and reports nothing); max_len is the longest
+ * sequence, and only steers how the work is split.  The result does
  * not depend on the order in which CTAs run.  `workspace` is device memory of
  * tb_kv4_attention_workspace bytes for the same arguments on the current
  * device (may be NULL if that is 0); it holds nothing between calls, and calls
