@@ -338,8 +338,39 @@ __device__ __forceinline__ PromptRow prompt_row(const Kv4Attn& a, const PromptUn
     return p;
 }
 
+// Rare: the blocks of 16 values d in which a row at position pos sees a NaN of V
+// that was left out of the products: those of tiles that the unit's rows do not
+// all see whole.  (All tiles looked through, a chunk of 8192 packed rows behind
+// 262144 tokens took 58.6 ms with one NaN at its end, 8.0 ms like this, as without it.)
+template <int D>
+__device__ __noinline__ uint32_t prompt_nan_blocks(const Kv4Attn& a, const int* list, int seqs, int item, int pos) {
+    const PromptUnit u = prompt_unit(a, list, seqs, item);
+    const int shift = a.cache.page_shift, gshift = shift < 7 ? shift : 7;
+    const int* table = a.rows.table + static_cast<size_t>(u.b) * a.rows.width;
+    uint32_t found = 0;
+    for (int j = u.t0; j < u.t1; ++j) {
+        const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
+        uint32_t pages = 0;  // as prompt_pages gives them
+        for (int k = 0; k < (kPromptTile >> gshift); ++k) {
+            const int tok = tok0 + (k << gshift);
+            if (tok < u.q.len && kv4_page_ok(a.cache, table[tok >> shift])) pages |= 1u << k;
+        }
+        if (prompt_open(a, u, tok0, pages)) continue;
+        for (int k = 0; k < kPromptTile; ++k) {
+            const int tok = tok0 + k;
+            if (!((pages >> (k >> gshift)) & 1u) || tok >= u.q.len || !kv4_sees(pos, tok, a.window, a.sinks)) continue;
+            const uint8_t* sc = a.cache.data + kv4_block_offset(a.cache, table[tok >> shift], u.head) +
+                                2 * kv4_codes_bytes(a.cache) + kv4_scales_bytes(a.cache) +
+                                (tok & ((1 << shift) - 1)) * (D / 16);
+            for (int x = 0; x < D / 16; ++x)
+                if ((sc[x] & 0x7F) == 0x7F) found |= 1u << x;
+        }
+    }
+    return found;
+}
+
 template <class C, bool BF16, bool DRAWN>
-__global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn a) {
+__global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const __grid_constant__ Kv4Attn a) {
     constexpr int D = C::D;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -564,24 +595,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv4_prompt(const Kv4Attn 
             if (!ok) break;
             tc_fence_after();
             uint32_t nan_blocks = 0;
-            if (*nan_seen && row.valid) {
-                // Rare: look at every block of V that was left out of a
-                // partly visible tile, and put a NaN where this row sees it.
-                for (int j = u.t0; j < u.t1; ++j) {
-                    const int tok0 = kv4_span_chunk(u.span, j) * kPromptTile;
-                    for (int k = 0; k < kPromptTile; ++k) {
-                        const int tok = tok0 + k;
-                        if (tok >= u.q.len || !kv4_sees(pos, tok, a.window, a.sinks)) continue;
-                        const int pg = a.rows.table[static_cast<size_t>(u.b) * a.rows.width + (tok >> a.cache.page_shift)];
-                        if (!kv4_page_ok(a.cache, pg)) continue;
-                        const uint8_t* sc = a.cache.data + kv4_block_offset(a.cache, pg, u.head) +
-                                            2 * kv4_codes_bytes(a.cache) + kv4_scales_bytes(a.cache) +
-                                            (tok & ((1 << a.cache.page_shift) - 1)) * (D / 16);
-                        for (int x = 0; x < D / 16; ++x)
-                            if ((sc[x] & 0x7F) == 0x7F) nan_blocks |= 1u << x;
-                    }
-                }
-            }
+            if (*nan_seen && row.valid) nan_blocks = prompt_nan_blocks<D>(a, list, seqs, item, pos);
             const bool partial = a.prompt_splits > 1;
             const float g = partial ? 1.0f : l == 0.0f ? 0.0f : a.cache.v_scale / l;
             // The warp's 32 rows go through its part of the query tile (whose

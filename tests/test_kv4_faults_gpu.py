@@ -79,3 +79,38 @@ def test_no_rows_by_max_rows(tb, cuda):
         out, lse = bt.attend(q, 2, 0.1, max_rows=0, max_len=max_len)
         assert bool((out == 7).all()) and bool((lse == 7).all())
         assert tb.device_error() == 0
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("typ,q_heads", [("f16", 1), ("bf16", 3)])
+def test_nan_values_in_whole_and_partly_seen_tiles(tb, cuda, typ, q_heads, page):
+    """NaN blocks of V in tiles of 128 tokens that all rows see whole, in those
+    that they see in part, and in one that has a page missing: each row has a NaN
+    where it sees one, and only there."""
+    n, lens = 300, [1500, 1000]
+    bt = Batch(tb, cuda, lens, [n, n], page=page, heads=1, dim=64, typ=typ, seed=page)
+    bt.fill_fast()
+    missing = 512 // page  # of sequence 0
+    bad = {0: [(200, 0), (700, 1), (1205, 2), (1350, 1), (1499, 3)], 1: [(0, 3), (701, 2), (999, 0)]}
+    if page == 16:
+        bad[0].append((530, 3))  # beside the missing page in its tile
+    for b, blocks in bad.items():
+        for pos, x in blocks:
+            pg, place = bt.place(b, pos)
+            ss = bt.host.parts(pg, 0, place, True)[1]
+            bt.host.data[pg, ss.start + x] = 0x7F
+    bt.upload()
+    bt.table[0, missing] = -1
+    bt.index()
+    q, _ = bt.queries(q_heads)
+    out, lse = bt.attend(q, q_heads, 0.1)
+    assert tb.device_error() == 2
+    assert bool(lse.isfinite().all())
+    o = out.float().cpu().numpy().reshape(-1, q_heads, 4, 16)
+    for b, blocks in bad.items():
+        for i in range(n):
+            pos = lens[b] - n + i
+            want = np.zeros(4, bool)
+            want[[x for p, x in blocks if p <= pos and not (b == 0 and p // page == missing)]] = True
+            got = np.isnan(o[bt.cu[b] + i])
+            assert np.array_equal(got, np.broadcast_to(want[None, :, None], got.shape)), (b, i)
