@@ -388,7 +388,7 @@ tb_status tb_kv4_read(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_for
  * with softmax_scale and softmax_scale * k_scale * log2(e) finite in FP32.
  * A row that sees nothing, or only scores of -inf, has out = 0, lse = -inf.
  * Sums and lse are FP32; the weights e^{s_j} are rounded to FP16 for the first
- * product, each by 2^-11 of itself or 2^-31 of the row's largest.
+ * product, each by 2^-11 of itself or 2^-30 of the row's largest.
  * max_rows is at least the rows of any sequence (with fewer, bit 2 of
  * tb_device_error's word is set and rows may be missing; 0 says that there are
  * none: the call does nothing and reports nothing); max_len is the longest

@@ -24,8 +24,8 @@
 // the converter second value first; Q is stored in the same order, and the
 // output's columns are swapped back when they are read.
 //
-// The maximum m of a row is moved only when a score passes it by 2^15, to 2^7
-// below that score, so the usual tile takes one pass: exponentials with the old
+// The maximum m of a row is moved only when a score passes it by almost 2^16, to
+// 2^6 below that score, so the usual tile takes one pass: exponentials with the old
 // m, the largest score found along the way, and a second pass (with O scaled in
 // TMEM) only if it passed.  S_t of a tile is issued behind
 // P_t V of the tile before, so a thread that sees S_t finds O_t at rest.
@@ -35,8 +35,8 @@
 // 2300: S_t waits for P_t V and P_t for S_t, so that the two tiles' phases
 // overlap only in part, and what the softmax warps issue beside the exponentials
 // (scale, maximum, sum, packing) shares its slots with the decoding warps.
-// P below 2^15 is rounded to FP16 as in the step kernel (m is a whole number here,
-// so P's largest may lie at 2^6), l is summed in FP32.
+// P is rounded to FP16 as in the step kernel (m is a whole number here, so P's
+// largest may lie at 2^5), l is summed in FP32.
 // Measured, 32 heads of 128, 8 KV heads: a prompt of 4096 tokens 162 us (848
 // TFLOP/s, 0.52 of a bf16 GEMM), 2048 rows behind 14336 tokens 544 us (950
 // TFLOP/s); ends of items cost ~14000 cycles each, hence whole rounds of large

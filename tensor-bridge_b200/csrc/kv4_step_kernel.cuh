@@ -21,13 +21,13 @@
 //     tokens are interleaved before they are converted (two operations for
 //     eight values), not the FP16 values after (four).
 //   - P^T's fragment is S^T's, transposed in 8 x 8 blocks: movmatrix.
-//   - the maximum is moved only when a score passes it by 2^15, and is then set
-//     2^7 below the largest score: P stays below 2^15, inside FP16, and the
+//   - the maximum is moved only when a score passes it by almost 2^16, and is
+//     then set 2^6 below the largest score: P stays inside FP16, and the
 //     reductions over lanes are rare.
-// P is rounded to FP16: by 2^-11 of itself down to 2^-21 of the row's largest
-// (P's largest is 2^7 at least), below that, where FP16 is subnormal, by up to
-// 2^-32 of the largest.  So where a row's weight lies on a few tokens of no value
-// the sum of the others is good to 1% while they are above 2^-25; with P at 1 at
+// P is rounded to FP16: by 2^-11 of itself down to 2^-20 of the row's largest
+// (P's largest is 2^6 at least), below that, where FP16 is subnormal, by up to
+// 2^-31 of the largest.  So where a row's weight lies on a few tokens of no value
+// the sum of the others is good to 1% while they are above 2^-24; with P at 1 at
 // most it was off by 13% at 2^-22 and all of it was lost at 2^-26.
 // l is summed from the FP32 values.
 //
@@ -85,9 +85,12 @@ constexpr int kStepChunk = 32;     // tokens of a warp's share of a tile
 // ordinary numbers; every score passes it.
 constexpr float kNoMax = -1e38f;
 // In log2 units: a score that passes the row's m by more than kPMost moves it, to
-// kPSet below the largest score.  P is then at most 2^7, far from the 2^-14 where
-// FP16 loses bits, and other scores may be 2^8 times larger until m moves again.
-constexpr float kPMost = 15.0f, kPSet = 7.0f;
+// kPSet below the largest score.  P is at most 2^15.9, below FP16's 65504, and its
+// largest at 2^6 when m has moved: higher, small weights keep more bits, but m
+// moves more often.  The prompt kernel's windowed chunks of 1500 rows (32 heads of
+// 64, window 2048) and prompt of 4096 tokens, a call: kPSet 4 151, 177 us; 5 160,
+// 177; 6 171, 178; 7 190, 181; 7 with kPMost 15 212, 190.
+constexpr float kPMost = 15.9f, kPSet = 6.0f;
 constexpr int kStepRowsMost = 32;  // packed rows of a (sequence, KV head)
 
 // NT tiles of eight rows.  Eight computing warps, and twelve for two tiles,

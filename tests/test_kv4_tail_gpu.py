@@ -19,10 +19,12 @@ def test_small_weights_behind_a_first_token(tb, cuda, n, dim, gap, max_len):
     """All tokens but the first weigh 2^-gap of it; its value is zero, theirs
     positive.
 
-    The bound: P is held in FP16 with the row's largest at 2^6 to 2^15, so a
+    The bound: P is held in FP16 with the row's largest at 2^6 or above, so a
     weight of 2^-gap of the largest is at 2^(6 - gap) or above and off by at most
     half a step, 2^-11 of itself or 2^-25 (FP16's subnormal steps are 2^-24), which
-    is 2^(gap - 31) of itself.  The other terms are those of kv4_oracle.tolerances."""
+    is 2^(gap - 31) of itself.  (From 33 packed rows on the largest may be at 2^5,
+    but there the small weights are powers of two here, and exact.)  The other
+    terms are those of kv4_oracle.tolerances."""
     bt = Batch(tb, cuda, [n + 99, n + 420], [n, n], page=16, heads=1, dim=dim, k_scale=1.0, v_scale=2.0 ** 16, seed=n + dim)
     for b, length in enumerate(bt.lens):
         for pos in range(length):
