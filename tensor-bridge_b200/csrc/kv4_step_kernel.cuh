@@ -81,9 +81,10 @@ struct Kv4Attn {
 enum : int { kErrRows = 4 };
 
 constexpr int kStepChunk = 32;     // tokens of a warp's share of a tile
-// A row's maximum before it has seen a score: finite, so that differences are
-// ordinary numbers; every score passes it.
-constexpr float kNoMax = -1e38f;
+// A row's maximum before it has seen a score: finite, so that a hidden score less
+// it is -inf and not NaN, and so low that every score passes it (a difference that
+// overflows does too).
+constexpr float kNoMax = -3.402823466e38f;
 // In log2 units: a score that passes the row's m by more than kPMost moves it, to
 // kPSet below the largest score.  P is at most 2^15.9, below FP16's 65504, and its
 // largest at 2^6 when m has moved: higher, small weights keep more bits, but m

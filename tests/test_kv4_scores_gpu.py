@@ -58,3 +58,32 @@ def test_infinite_query_beside_large_ones(tb, cuda, n, max_len):
         assert bool((out[row, 64 * head:64 * head + 64] == 0).all()) and lse[row, head].item() == -math.inf
         clean[row, 64 * head:64 * head + 64], clean_lse[row, head] = 0, -math.inf
     assert cuda.equal(out, clean) and cuda.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("max_len", [None, LONG])
+@pytest.mark.parametrize("size", [-1.6e38, 1.6e38])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_scores_near_the_ends_of_fp32(tb, cuda, n, size, max_len):
+    """All scores of a row are the same number, near an end of FP32's range: the
+    output is the mean of the values seen, lse that number.  The products are
+    sums of 64 equal terms and differ in no bit, so neither do the weights; the
+    mean takes FP16's half step for each weight, FP32 sums and BF16's half step."""
+    bt = Batch(tb, cuda, [n + 60, n + 700], [n, n], page=16, heads=1, dim=64, typ="bf16", k_scale=1.0, seed=n)
+    bt.fill_fast()
+    for page in range(bt.host.pages):
+        bt.host.data[page, :bt.host.codes] = 0x22
+        bt.host.data[page, bt.host.codes:bt.host.codes + bt.host.scales] = 0x38
+    bt.upload()
+    q, _ = bt.queries(2)
+    q.fill_(math.copysign(2.0 ** 115, size))
+    scale = abs(size) / 2.0 ** 121
+    out, lse = bt.attend(q, 2, scale, max_len=max_len)
+    o, ls = out.double().cpu().numpy().reshape(bt.total, 2, 64), lse.double().cpu().numpy()
+    for b in range(2):
+        v = bt.tokens(b, True)[:, 0]
+        for i in range(n):
+            seen = v[:bt.lens[b] - n + i + 1]
+            want, mass = seen.mean(axis=0), abs(seen).mean(axis=0)
+            tol = (2.0 ** -11 + 2.0 ** -20 + len(seen) * 2.0 ** -23) * mass + 2.0 ** -8 * abs(want)
+            assert (abs(o[bt.cu[b] + i] - want) <= tol).all(), (b, i)
+            assert (abs(ls[bt.cu[b] + i] - size) <= 2.0 ** -20 * abs(size)).all(), (b, i)
