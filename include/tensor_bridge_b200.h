@@ -388,7 +388,9 @@ tb_status tb_kv4_read(const tb_kv4_cache* cache, const tb_kv4_rows* rows, tb_for
  * with softmax_scale and softmax_scale * k_scale * log2(e) finite in FP32.
  * A row that sees nothing, or only scores of -inf, has out = 0, lse = -inf.
  * Sums and lse are FP32; the weights e^{s_j} are rounded to FP16 for the first
- * product, each by 2^-11 of itself or 2^-30 of the row's largest.
+ * product, each by 2^-11 of itself or 2^-30 of the row's largest.  A BF16 row of
+ * q is taken as FP16 times a power of two: exact for values down to 2^-28 of its
+ * largest, below that off by at most 2^-39 of the largest.
  * max_rows is at least the rows of any sequence (with fewer, bit 2 of
  * tb_device_error's word is set and rows may be missing; 0 says that there are
  * none: the call does nothing and reports nothing); max_len is the longest

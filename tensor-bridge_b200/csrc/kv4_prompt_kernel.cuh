@@ -34,13 +34,18 @@
 // cycles of an SM's exponentials and 1024 of its tensor core, and takes about
 // 2300: S_t waits for P_t V and P_t for S_t, so that the two tiles' phases
 // overlap only in part, and what the softmax warps issue beside the exponentials
-// (scale, maximum, sum, packing) shares its slots with the decoding warps.
+// (scale, maximum, sum, packing) shares its slots with the decoding warps.  At
+// D = 64 a tile takes hardly less, though its products are half: the softmax
+// warps' chain (wait, load, scale, maximum, exponential, pack, store) is what
+// remains, and each move of m, two passes more and O scaled, adds to it.
 // P is rounded to FP16 as in the step kernel (m is a whole number here, so P's
 // largest may lie at 2^5), l is summed in FP32.
-// Measured, 32 heads of 128, 8 KV heads: a prompt of 4096 tokens 162 us (848
-// TFLOP/s, 0.52 of a bf16 GEMM), 2048 rows behind 14336 tokens 544 us (950
-// TFLOP/s); ends of items cost ~14000 cycles each, hence whole rounds of large
-// items first.
+// Measured, 32 heads of 128, 8 KV heads, in a CUDA graph with the cache in L2: a
+// prompt of 4096 tokens 162 us (848 TFLOP/s, 0.52 of a bf16 GEMM; a call with L2
+// cold 176 us, 781 TFLOP/s), 2048 rows behind 14336 tokens 542 us (951 TFLOP/s;
+// with a CTA an item instead of persistent ones it took 493 us, the prompt as
+// long); ends of items cost ~14000 cycles each, hence whole rounds of large items
+// first.
 //
 // TMEM (512 columns): S_0, S_1 (128 each, P in the first 64), O_0, O_1 (D each).
 #pragma once

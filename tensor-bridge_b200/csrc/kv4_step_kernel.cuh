@@ -8,7 +8,9 @@
 //
 // What bounds it: 18 D / 16 bytes a token and KV head come from memory, and
 // an SM has about six cycles for the 144 bytes of D = 128.  In those it must
-// turn 256 codes into FP16 and multiply them, so instructions count:
+// turn 256 codes into FP16 and multiply them, so instructions count (issue slots
+// are 60% full, and the conversions and half-precision products, two cycles
+// each, are what the warps wait for beside fixed latencies):
 //   - S^T = K Q^T and O^T = V^T P^T put tokens (d) on the 16-row side of
 //     mma.m16n8k16 and the rows r on its 8 columns: eight rows, the usual size
 //     of a group, cost half of what padding them to 16 would.  (tcgen05.mma
@@ -33,7 +35,9 @@
 //
 // BF16 queries are scaled per row by a power of two to at most 2^15 and taken
 // as FP16: exact for values within 2^-28 of the row's largest, and off by at
-// most 2^-39 of it below, which FP32 sums do not resolve.
+// most 2^-39 of it below.  FP32 sums do not resolve that where the largest meets
+// a key that is not zero; where it meets only zeros, queries below 2^-40 of it
+// are lost from the scores.
 //
 // Split: the (sequence, KV head) units' chunks are laid end to end, and each
 // CTA takes an equal run of them, so a batch of any lengths loads all SMs
@@ -45,10 +49,10 @@
 // goes on into the next unit while the other warps compute, each on its own 32
 // tokens of a tile with its own o, m, l, merged once per unit in a fixed order.
 //
-// Measured, 8 KV heads of 128, one row: 4 sequences of 65536 tokens, 64 heads,
-// 67.8 us (4.45 TB/s, 0.68 of a copy; about 10 us of it are the start and the
-// ends of the runs, the rest goes at 0.72); 32 of 4000, 32 heads, 42 us; 1 of
-// 1000 7.4 us.  20 packed rows (three tiles of 8), 8 of 10000: 47 us.
+// Measured in a CUDA graph, 8 KV heads of 128, one row: 4 sequences of 65536
+// tokens, 64 heads, 68.0 us (4.44 TB/s, 0.68 of a copy; about 10 us of it are the
+// start and the ends of the runs, the rest goes at 0.72); 32 of 4000, 32 heads,
+// 42 us; 1 of 1000 7.5 us.  20 packed rows (three tiles of 8), 8 of 10000: 48 us.
 #pragma once
 
 #include "kv4_cache_kernel.cuh"
